@@ -245,6 +245,109 @@ int race_fwd_noalloc(const race_desc *d, const void *q, const void *k, const voi
  * descriptor's inv_temp_ptr. */
 int race_inv_temp(const float *logit, float lo, float hi, float *out, void *stream);
 
+/* ---------------------------------------------------------------------
+ * The operators around RACE attention in its blocks: root-mean-square norm,
+ * linear layers in 8 bits, AdamW.  No counterpart in the reference, whose
+ * blocks use LayerNorm, torch's linear layers and torch's AdamW; same rules as
+ * above (caller's buffers and stream, no allocation, deterministic).  Strides
+ * are in elements between rows; columns are contiguous; rows start at any
+ * multiple of their element's size.
+ * --------------------------------------------------------------------- */
+
+/* Root-mean-square norm with the residual's addition:
+ *   h = x + residual (h = x without one),  rstd = 1 / sqrt(mean(h^2) + eps),  y = h rstd w.
+ * x, y and their gradients have type dtype, residual, h and theirs r_dtype (the same, or fp32
+ * beside a bf16 x); w, rstd, dw are fp32.  h is rounded where it is stored, y normalises the
+ * unrounded sum. */
+typedef struct race_norm_desc {
+    int64_t rows, D;
+    int64_t x_stride, r_stride, y_stride, h_stride;     /* forward */
+    int64_t dy_stride, dh_stride, dx_stride, dr_stride; /* backward (with x_stride, r_stride) */
+    int32_t dtype, r_dtype;
+    float eps;
+} race_norm_desc;
+
+/* residual and h are given together or not at all; rstd [rows] (nullable) is for the backward. */
+int race_rms_norm(const race_norm_desc *d, const void *x, const void *residual, const float *w,
+                  void *y, void *h, float *rstd, void *stream);
+
+/* The sum is x + residual, or where x is NULL residual alone: the forward's x without a
+ * residual, or its fp32 h.  dh, the gradient of h beside y's, is nullable; dx = dresidual,
+ * rounded to either type, where not NULL. */
+size_t race_rms_norm_bwd_workspace_bytes(const race_norm_desc *d);
+int race_rms_norm_bwd(const race_norm_desc *d, const void *x, const void *residual, const float *w,
+                      const float *rstd, const void *dy, const void *dh, void *dx, void *dresidual, float *dw,
+                      void *ws, size_t ws_bytes, void *stream);
+
+/* A matrix in 8-bit blocks: value [r][c] = code * 2^(scale byte - 127), codes e4m3 (OCP), one
+ * scale byte (e8m0) for 128 columns of block_rows rows: scale[r / block_rows][c / 128].  Blocks
+ * at the end of a row or of the rows may be short.  A quantiser's scale is the least power of
+ * two with amax / 2^s <= 448 (1 for a block of zeros), amax over the block's finite values;
+ * what is not finite becomes a NaN code.  A scale byte of 255 (NaN) makes its products NaN. */
+typedef struct race_blocks {
+    void *codes;          /* [rows][ld] bytes */
+    void *scale;          /* [ceil(rows / block_rows)][scale_ld] bytes */
+    int64_t rows, cols;
+    int64_t ld, scale_ld; /* row pitches */
+    int32_t block_rows;   /* 1 or 128 */
+} race_blocks;
+
+/* The norm's y in 8-bit blocks (block_rows = 1), with pitch and codes as race_quantize. */
+int race_rms_norm_codes(const race_norm_desc *d, const void *x, const void *residual, const float *w,
+                        const race_blocks *y, void *h, void *stream);
+
+/* x [rows][cols] in 8-bit blocks: y of x, yt of its transpose (each nullable, not both; the
+ * same block_rows), and sums [cols] (nullable): x's column sums in fp32.  x is read once.
+ * Codes start at a multiple of 16 bytes and their pitch is one that holds the columns rounded
+ * up to 16, which are written (zeros behind the last).  ws: for the sums alone. */
+size_t race_quantize_workspace_bytes(int64_t rows, int64_t cols);
+int race_quantize(const void *x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld,
+                  const race_blocks *y, const race_blocks *yt, float *sums, void *ws,
+                  size_t ws_bytes, void *stream);
+
+/* out [a.rows][b.rows] = a b^T + bias (nullable), of type out_dtype.  An fp32 output is summed
+ * in fp32; a bf16 one by the 8-bit matrix instructions, whose sums of 128 products are about
+ * 2e-5 of their norm off (a bf16 step: 4e-3).  Codes
+ * of any pitch and alignment; those that are whole 16-byte pieces are read in place, others are
+ * copied to the workspace first (a of more than race_block_linear_rows() rows).  Workspace 0: ws
+ * may be NULL. */
+size_t race_block_matmul_workspace_bytes(const race_blocks *a, const race_blocks *b, int32_t out_dtype);
+int race_block_matmul(const race_blocks *a, const race_blocks *b, const float *bias, void *out,
+                      int32_t out_dtype, int64_t out_ld, void *ws, size_t ws_bytes, void *stream);
+
+/* The same for 1 to race_block_linear_rows() rows of x in bf16 or fp32, quantised on the way as
+ * race_quantize with block_rows = 1 does: a linear layer's single tokens in one launch. */
+int64_t race_block_linear_rows(void);
+size_t race_block_linear_workspace_bytes(int64_t rows, const race_blocks *b, int32_t out_dtype);
+int race_block_linear(const void *x, int32_t dtype, int64_t rows, int64_t x_ld, const race_blocks *b,
+                      const float *bias, void *out, int32_t out_dtype, int64_t out_ld, void *ws,
+                      size_t ws_bytes, void *stream);
+
+/* One AdamW step over count tensors of n contiguous elements each:
+ *   m = beta_m m + (1 - beta_m) g,  v = beta_v v + (1 - beta_v) g^2,
+ *   p = p - lr weight_decay p - lr / (1 - beta_m^t) m / (sqrt(v) / sqrt(1 - beta_v^t) + eps).
+ * bits = 32: m and v fp32.  bits = 8: m and sqrt(v) as e4m3 codes with a scale byte for each 128
+ * elements (m_scale, v_scale; as race_blocks), rounded stochastically: element j of tensor i has
+ * the place j + sum of the earlier tensors' n, each rounded up to 128, and the random number
+ * mix(place + mix(seed)) mod 2^32, whose low half rounds m and high half sqrt(v).  (A state of
+ * zeros: zero codes.)  p may be bf16, then rounded to the nearest.  step_ptr (nullable): t as a
+ * device fp32 scalar read when the kernels run, for captured graphs; step is not used then, and
+ * seed + t takes seed's place. */
+typedef struct race_adamw_tensor {
+    void *p;
+    const void *g;
+    void *m, *v;
+    void *m_scale, *v_scale; /* bits = 8 */
+    int64_t n;
+} race_adamw_tensor;
+typedef struct race_adamw_desc {
+    double lr, beta_m, beta_v, eps, weight_decay, step;
+    const float *step_ptr;
+    uint32_t seed;
+    int32_t bits, p_dtype, g_dtype;
+} race_adamw_desc;
+int race_adamw(const race_adamw_desc *d, const race_adamw_tensor *t, int64_t count, void *stream);
+
 /* Message for the last failing call on this thread ("" if none). */
 const char *race_last_error(void);
 

@@ -40,6 +40,32 @@ class RaceDesc(ctypes.Structure):
     ]
 
 
+class NormDesc(ctypes.Structure):
+    """Mirror of race_norm_desc."""
+    _fields_ = [(n, ctypes.c_int64) for n in ("rows", "D", "x_stride", "r_stride", "y_stride", "h_stride", "dy_stride",
+                                              "dh_stride", "dx_stride", "dr_stride")] + [
+        ("dtype", ctypes.c_int32), ("r_dtype", ctypes.c_int32), ("eps", ctypes.c_float)]
+
+
+class Blocks(ctypes.Structure):
+    """Mirror of race_blocks."""
+    _fields_ = [("codes", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("rows", ctypes.c_int64),
+                ("cols", ctypes.c_int64), ("ld", ctypes.c_int64), ("scale_ld", ctypes.c_int64),
+                ("block_rows", ctypes.c_int32)]
+
+
+class AdamwTensor(ctypes.Structure):
+    """Mirror of race_adamw_tensor."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("p", "g", "m", "v", "m_scale", "v_scale")] + [("n", ctypes.c_int64)]
+
+
+class AdamwDesc(ctypes.Structure):
+    """Mirror of race_adamw_desc."""
+    _fields_ = [(n, ctypes.c_double) for n in ("lr", "beta_m", "beta_v", "eps", "weight_decay", "step")] + [
+        ("step_ptr", ctypes.c_void_p), ("seed", ctypes.c_uint32), ("bits", ctypes.c_int32),
+        ("p_dtype", ctypes.c_int32), ("g_dtype", ctypes.c_int32)]
+
+
 # every symbol include/race_attention.h declares
 EXPORTS = (
     "race_state_bytes", "race_fwd_workspace_bytes", "race_bwd_workspace_bytes",
@@ -51,6 +77,11 @@ EXPORTS = (
     "race_prefix_mean_workspace_bytes", "race_prefix_mean_fwd", "race_prefix_mean_bwd",
     "race_fwd_noalloc",
     "race_inv_temp",
+    "race_rms_norm", "race_rms_norm_codes", "race_rms_norm_bwd_workspace_bytes", "race_rms_norm_bwd",
+    "race_quantize_workspace_bytes", "race_quantize",
+    "race_block_matmul_workspace_bytes", "race_block_matmul",
+    "race_block_linear_rows", "race_block_linear_workspace_bytes", "race_block_linear",
+    "race_adamw",
     "race_last_error", "race_abi_version",
 )
 
@@ -107,12 +138,33 @@ def load():
         lib.race_fwd_noalloc.restype = ctypes.c_int
         lib.race_inv_temp.argtypes = [vp, ctypes.c_float, ctypes.c_float, vp, vp]
         lib.race_inv_temp.restype = ctypes.c_int
+        _declare_layers(lib)
         lib.race_last_error.argtypes = []
         lib.race_last_error.restype = ctypes.c_char_p
         lib.race_abi_version.argtypes = []
         lib.race_abi_version.restype = ctypes.c_int
         _lib = lib
         return lib
+
+
+def _declare_layers(lib):
+    """The operators around the attention."""
+    vp, sz, i64, i32 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int64, ctypes.c_int32
+    nd, bp, ad = ctypes.POINTER(NormDesc), ctypes.POINTER(Blocks), ctypes.POINTER(AdamwDesc)
+    for name, res, args in (
+            ("race_rms_norm", i32, [nd, vp, vp, vp, vp, vp, vp, vp]),
+            ("race_rms_norm_codes", i32, [nd, vp, vp, vp, bp, vp, vp]),
+            ("race_rms_norm_bwd_workspace_bytes", sz, [nd]),
+            ("race_rms_norm_bwd", i32, [nd, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]),
+            ("race_quantize_workspace_bytes", sz, [i64, i64]),
+            ("race_quantize", i32, [vp, i32, i64, i64, i64, bp, bp, vp, vp, sz, vp]),
+            ("race_block_matmul_workspace_bytes", sz, [bp, bp, i32]),
+            ("race_block_matmul", i32, [bp, bp, vp, vp, i32, i64, vp, sz, vp]),
+            ("race_block_linear_rows", i64, []),
+            ("race_block_linear_workspace_bytes", sz, [i64, bp, i32]),
+            ("race_block_linear", i32, [vp, i32, i64, i64, bp, vp, vp, i32, i64, vp, sz, vp]),
+            ("race_adamw", i32, [ad, ctypes.POINTER(AdamwTensor), i64, vp])):
+        getattr(lib, name).argtypes, getattr(lib, name).restype = args, res
 
 
 TORCH_PATH = os.path.join(HERE, "_race_torch.so")

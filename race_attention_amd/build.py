@@ -1,8 +1,9 @@
 """Build the gfx950 HIP library race_attention_amd/librace_attention.so and the
 autograd calls over it, race_attention_amd/_race_torch.so.
 
-The library is one translation unit (csrc/race_capi.hip, which includes the
-kernel sources) compiled with hipcc for gfx950 only.  Packed-fp32 instruction
+The library is two translation units compiled side by side with hipcc for gfx950
+only: csrc/race_capi.hip (the attention operators; it includes their kernel sources)
+and csrc/layers_capi.hip (the operators around them, likewise).  Packed-fp32 instruction
 selection is disabled (-packed-fp32-ops) for all device code.  The autograd
 calls (csrc/race_torch.cpp) are host code against torch's C++ API.
 """
@@ -10,9 +11,10 @@ import os
 import subprocess
 import sys
 import sysconfig
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SRC = os.path.join(HERE, "csrc", "race_capi.hip")
+SRCS = [os.path.join(HERE, "csrc", name) for name in ("race_capi.hip", "layers_capi.hip")]
 OUT = os.path.join(HERE, "librace_attention.so")
 TORCH_SRC = os.path.join(HERE, "csrc", "race_torch.cpp")
 TORCH_OUT = os.path.join(HERE, "_race_torch.so")
@@ -52,15 +54,32 @@ def build(verbose: bool = True, sanitize: bool = False) -> str:
                                 text=True)
     if sanitize:
         os.makedirs(os.path.dirname(out), exist_ok=True)
-    cmd = [HIPCC] + FLAGS + (SAN_FLAGS if sanitize else []) + [SRC, "-o", out + ".tmp"]
-    if verbose:
-        print("build:", " ".join(cmd), flush=True)
-    proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if proc.returncode != 0 and host is not None:
+    flags = FLAGS + (SAN_FLAGS if sanitize else [])
+    compile_flags = [f for f in flags if f != "-shared"]
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [os.path.join(tmp, os.path.basename(src) + ".o") for src in SRCS]
+        cmds = [[HIPCC] + compile_flags + ["-c", src, "-o", obj] for src, obj in zip(SRCS, objs)]
+        link = [HIPCC] + flags + objs + ["-o", out + ".tmp"]
+        if verbose:
+            for cmd in cmds + [link]:
+                print("build:", " ".join(cmd), flush=True)
+        # compiler output to files: the processes run side by side, and a full pipe would stop one
+        logs = [open(obj + ".log", "w+") for obj in objs]
+        procs = [subprocess.Popen(cmd, stdout=log, stderr=subprocess.STDOUT) for cmd, log in zip(cmds, logs)]
+        rc = max([abs(p.wait()) for p in procs])
+        text = ""
+        for log in logs:
+            log.seek(0)
+            text += log.read()
+            log.close()
+        if rc == 0:
+            proc = subprocess.run(link, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+            rc, text = proc.returncode, text + proc.stdout
+    if rc != 0 and host is not None:
         host.kill()
         host.wait()
-    msgs = [ln for ln in proc.stdout.splitlines() if "packed-fp32-ops" not in ln]
-    if proc.returncode != 0:
+    msgs = [ln for ln in text.splitlines() if "packed-fp32-ops" not in ln]
+    if rc != 0:
         print("\n".join(msgs), file=sys.stderr)
         raise RuntimeError("hipcc failed building librace_attention.so")
     if verbose and msgs:

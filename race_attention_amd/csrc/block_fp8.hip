@@ -1,0 +1,519 @@
+// block_fp8.hip -- gfx950 kernels of matrices in 8-bit blocks: the quantiser and the
+// product out = a b^T of two of them.
+//
+// A matrix [rows][cols] in 8-bit blocks: e4m3 codes and a power-of-two scale for each
+// block of 128 columns of one row (activations) or of 128 columns of 128 rows
+// (weights).  With S_a, S_b the scales' exponents,
+//   out[m][n] = sum_kb 2^(S_a[m,kb] + S_b[n,kb]) sum_{k in block kb} a[m,k] b[n,k].
+// v_mfma_scale_f32_16x16x128_f8f6f4 contracts 128 codes and takes a scale byte for
+// every row of both operands, so one instruction is one block of a 16x16 tile, without
+// any work on the vector units.
+//
+// The 8-bit matrix instructions (of any depth) add their products with few bits: what is
+// under 2^-18 of the largest is lost, and sums of 128 random products are 1.7e-5 of
+// their norm off.  That is far under half a step of a bf16 result (2^-9), but not of an
+// fp32 one, which is asked for where many products are summed (the weights' gradient).  So
+// products with an fp32 output turn the codes into bf16 on the way to the matrix cores
+// (v_cvt_scalef32_pk_bf16_fp8 applies the scale; both are exact) and use the bf16
+// instructions, which sum in fp32 at half the rate.
+#include "layers.h"
+
+namespace race {
+
+// ------------------------------------------------------------ quantiser
+struct QuantArgs {
+    const void *x;
+    int64_t rows, cols, ld;
+    uint8_t *codes, *scale;      // [rows][cols], nullable
+    int64_t codes_ld, scale_ld;
+    uint8_t *codes_t, *scale_t;  // of the transpose, [cols][rows], nullable
+    int64_t codes_t_ld, scale_t_ld;
+    float *sums;                 // [ceil(rows / 128)][cols] column sums of 128 rows, nullable
+};
+
+// Rows alone: 16 lanes hold a block of 128 columns.  Bound by memory; 16 blocks a
+// workgroup, so that a batch of few rows is spread over the chip.
+template <typename T> __global__ __launch_bounds__(256) void k_quantize_rows(QuantArgs a) {
+    const int64_t nb = (a.cols + BLK - 1) / BLK, total = a.rows * nb;
+    const int l = threadIdx.x & 15;
+    for (int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); i < total; i += (int64_t)gridDim.x * 16) {
+        const int64_t row = i / nb, kb = i % nb, c = kb * BLK + 8 * l;
+        float v[8], amax = 0.f;
+        ld_row<T, 8>((const T *)a.x + row * a.ld, c, a.cols, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(v[j]));
+        const int b = scale_byte(row16(amax, Max{}));
+        st_codes<8>(a.codes + row * a.codes_ld, c, a.codes_ld < nb * BLK ? a.codes_ld : nb * BLK, v, inv_scale(b));
+        if (l == 0) a.scale[row * a.scale_ld + kb] = (uint8_t)b;
+    }
+}
+
+// A 128 x 128 tile, read once, for any of: the row-wise blocks, the blocks of the
+// transpose (128 rows of one column), one block of both (BLOCK), and the column sums.
+// Thread (i, l) = (tid / 16, tid % 16) holds 8 rows x 8 columns: the amax of a row is
+// one over 16 neighbouring lanes, that of a column one over the 8 rows in registers,
+// then over the 16 threads above each other through LDS.  Transposed codes leave through
+// LDS in rows of 128 bytes.
+template <typename T, bool BLOCK>
+__global__ __launch_bounds__(256) void k_quantize_tile(QuantArgs a) {
+    __shared__ float red[16][BLK];
+    __shared__ uint32_t tr[BLK * 33];  // [column][32 words of 4 rows], pitch 33
+    const int l = threadIdx.x & 15, i = threadIdx.x >> 4;
+    const int64_t r0 = (int64_t)blockIdx.y * BLK, c0 = (int64_t)blockIdx.x * BLK;
+    const int64_t c = c0 + 8 * l;
+    float v[8][8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        const int64_t row = r0 + 8 * i + r;
+        if (row < a.rows) {
+            ld_row<T, 8>((const T *)a.x + row * a.ld, c, a.cols, v[r]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[r][j] = 0.f;
+        }
+    }
+    int bt[8];  // scale bytes of the transposed blocks of this thread's 8 columns
+    int ball = 0;
+    if (BLOCK || a.codes_t) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float m = 0.f;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) m = fmaxf(m, finite_abs(v[r][j]));
+            red[i][8 * l + j] = m;
+        }
+        __syncthreads();
+        float all = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float m = 0.f;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) m = fmaxf(m, red[k][8 * l + j]);
+            bt[j] = scale_byte(m);
+            all = fmaxf(all, m);
+        }
+        if constexpr (BLOCK) ball = scale_byte(row16(all, Max{}));
+        __syncthreads();
+    }
+    const int64_t cend = a.codes_ld < a.cols + (-a.cols & 15) ? a.codes_ld : a.cols + (-a.cols & 15);
+    if (a.codes) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int64_t row = r0 + 8 * i + r;
+            int b = ball;
+            if constexpr (!BLOCK) {
+                float m = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(v[r][j]));
+                b = scale_byte(row16(m, Max{}));
+            }
+            if (row < a.rows) {
+                st_codes<8>(a.codes + row * a.codes_ld, c, cend, v[r], inv_scale(b));
+                if (!BLOCK && l == 0) a.scale[row * a.scale_ld + blockIdx.x] = (uint8_t)b;
+            }
+        }
+        if (BLOCK && threadIdx.x == 0) a.scale[blockIdx.y * a.scale_ld + blockIdx.x] = (uint8_t)ball;
+    }
+    if (a.codes_t) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float inv = inv_scale(BLOCK ? ball : bt[j]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                tr[(8 * l + j) * 33 + 2 * i + h] = codes4(v[4 * h][j] * inv, v[4 * h + 1][j] * inv,
+                                                          v[4 * h + 2][j] * inv, v[4 * h + 3][j] * inv);
+            if (!BLOCK && i == 0 && c + j < a.cols) a.scale_t[(c + j) * a.scale_t_ld + blockIdx.y] = (uint8_t)bt[j];
+        }
+        if (BLOCK && threadIdx.x == 0) a.scale_t[blockIdx.x * a.scale_t_ld + blockIdx.y] = (uint8_t)ball;
+        __syncthreads();
+        // codes_t_ld is a multiple of 16: pieces of 16 rows, zeros behind the last row
+        for (int p = threadIdx.x; p < BLK * 8; p += 256) {
+            const int col = p >> 3, piece = p & 7;
+            if (c0 + col < a.cols && r0 + 16 * piece < a.codes_t_ld) {
+                uint32_t q[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) q[k] = tr[col * 33 + 4 * piece + k];
+                __builtin_memcpy(a.codes_t + (c0 + col) * a.codes_t_ld + r0 + 16 * piece, q, 16);
+            }
+        }
+    }
+    if (a.sums) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float s = 0.f;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) s += v[r][j];
+            red[i][8 * l + j] = s;
+        }
+        __syncthreads();
+        if (threadIdx.x < BLK && c0 + threadIdx.x < a.cols) {
+            float s = 0.f;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) s += red[k][threadIdx.x];
+            a.sums[(int64_t)blockIdx.y * a.cols + c0 + threadIdx.x] = s;
+        }
+    }
+}
+
+// Codes [rows][cols] of any pitch and alignment to a pitch that is a multiple of 16, zeros behind
+// the last column.
+__global__ __launch_bounds__(256) void k_repack(const uint8_t *__restrict__ x, int64_t rows, int64_t cols, int64_t ld,
+                                                uint8_t *__restrict__ y, int64_t y_ld) {
+    const int64_t np = y_ld / 16, total = rows * np;
+    for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < total; p += (int64_t)gridDim.x * 256) {
+        const int64_t row = p / np, c = p % np * 16;
+        uint8_t q[16];
+        if (c + 16 <= cols) {
+            __builtin_memcpy(q, x + row * ld + c, 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) q[j] = c + j < cols ? x[row * ld + c + j] : 0;
+        }
+        __builtin_memcpy(y + row * y_ld + c, q, 16);
+    }
+}
+
+// ------------------------------------------------------------ product
+struct MatArgs {
+    const uint8_t *a, *b;    // codes [M][K], [N][K]; pitches and K multiples of 16 for the tile kernels
+    const uint8_t *sa, *sb;  // scale bytes
+    const float *bias;       // [N], nullable
+    void *out;
+    float *part;             // [splits][M][N] where the contraction is split
+    int64_t M, N, K, lda, ldb, lsa, lsb, ldo;
+    int sha, shb;            // log2 of the rows that share a scale: 0 or 7
+    int ksteps;              // blocks of 128 along K
+    int kper;                // of them for each split
+    int tm, tn;              // tiles
+};
+
+typedef __attribute__((address_space(3))) char lds_char;
+
+// Granule (16 bytes) g of row r of an LDS tile of 128-byte rows stands at g ^ swz(r).
+// A fragment is two ds_read_b128 of granules q and q + 4, q = lane / 16 (the order of k
+// inside a block is free, as long as both operands have the same): with bits 1..3 of the
+// row in the swizzle, the 16 lanes of each of its passes ({0-3, 12-15, 20-27} and so on:
+// rows 0-3, 12-15 of one granule and 4-11 of its neighbour) fall on 16 different
+// 16-byte banks.
+__device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
+
+// Tile of R rows: direct loads from memory to LDS, 16 bytes a lane, 8 rows a wave and
+// instruction; what lies behind the matrix reads as zeros (its offset is out of the
+// buffer's range).
+template <int R, int WAVES>
+__device__ __forceinline__ void stage(const uint8_t *base, int64_t ld, int64_t rows_left, int64_t K, int kb,
+                                      char *lds, int wave, int lane) {
+    const int64_t rows = rows_left < R ? rows_left : R;
+    // whole rows below 2^31 bytes: checked by the caller
+    __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t *>(base), 0, (int)((rows - 1) * ld + K), 0x00027000);
+    const int rl = lane >> 3, g = lane & 7;
+#pragma unroll
+    for (int i = 0; i < R / 8 / WAVES; ++i) {
+        const int r0 = (i * WAVES + wave) * 8, r = r0 + rl;
+        const int64_t k = (int64_t)kb * BLK + 16 * (g ^ swz(r));
+        const int off = r < rows && k < K ? (int)(r * ld + k) : 0x7fffffff;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void *)(lds + r0 * BLK), 16,
+                                                 off, 0, 0, 0);
+    }
+}
+
+__device__ __forceinline__ i32x8 fragment(const char *lds, int row, int q) {
+    const i32x4 lo = *(const i32x4 *)(lds + row * BLK + 16 * (q ^ swz(row)));
+    const i32x4 hi = *(const i32x4 *)(lds + row * BLK + 16 * ((q + 4) ^ swz(row)));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// One block of a 16x16 tile: c += 2^(sa + sb) a b^T for lanes' fragments fb (rows of b: the
+// tile's rows) and fa (rows of a: its columns).
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+struct Wide { bf16x8 v[4]; };  // 32 codes as bf16, their scale applied
+__device__ __forceinline__ Wide widen(const i32x8 &f, uint32_t s) {
+    const float scale = scale_of((int)(s & 255u));
+    Wide w;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)f[j], scale, false);
+        const bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)f[j], scale, true);
+        w.v[j / 2][4 * (j & 1)] = lo[0];
+        w.v[j / 2][4 * (j & 1) + 1] = lo[1];
+        w.v[j / 2][4 * (j & 1) + 2] = hi[0];
+        w.v[j / 2][4 * (j & 1) + 3] = hi[1];
+    }
+    return w;
+}
+__device__ __forceinline__ f32x4 block_product(const Wide &b, const Wide &a, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.v[j], a.v[j], c, 0, 0, 0);
+    return c;
+}
+struct Codes { i32x8 v; uint32_t s; };
+__device__ __forceinline__ f32x4 block_product(const Codes &b, const Codes &a, f32x4 c) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.v, a.v, c, 0, 0, 0, (int)b.s, 0, (int)a.s);
+}
+// a fragment as the product of an output type takes it
+template <typename TO> struct Operand {
+    typedef Codes type;
+    static __device__ __forceinline__ Codes of(const i32x8 &f, uint32_t s) { return Codes{f, s}; }
+};
+template <> struct Operand<float> {
+    typedef Wide type;
+    static __device__ __forceinline__ Wide of(const i32x8 &f, uint32_t s) { return widen(f, s); }
+};
+
+// four scale bytes kb .. kb+3 of a row, those from n on 0 (their codes are zeros)
+__device__ __forceinline__ uint32_t scales4(const uint8_t *row, int kb, int n) {
+    uint32_t s = 0;
+    if (kb + 4 <= n) {
+        __builtin_memcpy(&s, row + kb, 4);
+    } else {
+        for (int j = 0; j < 3; ++j)
+            if (kb + j < n) s |= (uint32_t)row[kb + j] << (8 * j);
+    }
+    return s;
+}
+
+template <typename TO> __device__ __forceinline__ void st_out4(TO *p, const f32x4 &v, int64_t left) {
+    const float t[4] = {v[0], v[1], v[2], v[3]};
+    if (left >= 4) {
+        st_vec<TO, 4>(p, t);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < left) p[j] = (TO)t[j];
+    }
+}
+
+// Workgroups go round the 8 XCDs in turn, each with an L2 of its own: an XCD takes a
+// contiguous run of tiles, in bands of 8 tile rows, so that the tiles it works on at a
+// time share their rows of a and of b.
+__device__ __forceinline__ void tile_of(int id, int tm, int tn, int &im, int &in) {
+    const int n = tm * tn, per = n / 8, rest = n % 8, xcd = id % 8, k = id / 8;
+    const int t = xcd * per + (xcd < rest ? xcd : rest) + k;
+    const int band = 8 * tn, b = t / band, h = tm - 8 * b < 8 ? tm - 8 * b : 8;
+    im = 8 * b + (t - b * band) % h;
+    in = (t - b * band) / h;
+}
+
+template <int BM, int BN, int WM, int WN, typename TO>
+__global__ __launch_bounds__(64 * WM * WN) void k_block_matmul(MatArgs a) {
+    constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
+    __shared__ __align__(16) char buf[2][(BM + BN) * BLK];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN, q = lane >> 4, i16 = lane & 15;
+    int im, in;
+    tile_of(blockIdx.x, a.tm, a.tn, im, in);
+    const int64_t m0 = (int64_t)im * BM, n0 = (int64_t)in * BN;
+    const int kb0 = blockIdx.y * a.kper, kb1 = kb0 + a.kper < a.ksteps ? kb0 + a.kper : a.ksteps;
+    const uint8_t *abase = a.a + m0 * a.lda, *bbase = a.b + n0 * a.ldb;
+    const uint8_t *srow_a[TM], *srow_b[TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int64_t m = m0 + (wm * TM + i) * 16 + i16;
+        srow_a[i] = a.sa + ((m < a.M ? m : a.M - 1) >> a.sha) * a.lsa;
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int64_t n = n0 + (wn * TN + j) * 16 + i16;
+        srow_b[j] = a.sb + ((n < a.N ? n : a.N - 1) >> a.shb) * a.lsb;
+    }
+    auto load = [&](int kb, char *to) {
+        stage<BM, WAVES>(abase, a.lda, a.M - m0, a.K, kb, to, wave, lane);
+        stage<BN, WAVES>(bbase, a.ldb, a.N - n0, a.K, kb, to + BM * BLK, wave, lane);
+    };
+    f32x4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    uint32_t sa[TM], sb[TN];
+    load(kb0, buf[0]);
+    for (int kb = kb0; kb < kb1; ++kb) {
+        const int cur = (kb - kb0) & 1;
+        if (((kb - kb0) & 3) == 0) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i) sa[i] = scales4(srow_a[i], kb, a.ksteps);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) sb[j] = scales4(srow_b[j], kb, a.ksteps);
+        }
+        __syncthreads();  // the tile of kb is in LDS; the other buffer's readers are done
+        if (kb + 1 < kb1) load(kb + 1, buf[cur ^ 1]);
+        const char *ta = buf[cur], *tb = ta + BM * BLK;
+        typename Operand<TO>::type fb[TN];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) fb[j] = Operand<TO>::of(fragment(tb, (wn * TN + j) * 16 + i16, q), sb[j]);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const typename Operand<TO>::type fa = Operand<TO>::of(fragment(ta, (wm * TM + i) * 16 + i16, q), sa[i]);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = block_product(fb[j], fa, acc[i][j]);
+        }
+#pragma unroll
+        for (int i = 0; i < TM; ++i) sa[i] >>= 8;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) sb[j] >>= 8;
+    }
+    // lane: column i16 of the product's tile (a row of a), rows 4q .. 4q+3 (rows of b)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int64_t n = n0 + (wn * TN + j) * 16 + 4 * q;
+        f32x4 bias = {0.f, 0.f, 0.f, 0.f};
+        if (a.bias && !a.part)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bias[e] = n + e < a.N ? a.bias[n + e] : 0.f;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const int64_t m = m0 + (wm * TM + i) * 16 + i16;
+            if (m >= a.M || n >= a.N) continue;
+            if (a.part)
+                st_out4<float>(a.part + ((int64_t)blockIdx.y * a.M + m) * a.N + n, acc[i][j], a.N - n);
+            else
+                st_out4<TO>((TO *)a.out + m * a.ldo + n, acc[i][j] + bias, a.N - n);
+        }
+    }
+}
+
+// The parts of a split contraction, added in order, with the bias.
+template <typename TO> __global__ __launch_bounds__(256) void k_split_sum(MatArgs a, int splits) {
+    const int64_t total = a.M * a.N, stride = (int64_t)gridDim.x * 256 * 4;
+    for (int64_t p = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; p < total; p += stride) {
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int z = 0; z < splits; ++z) {
+            float t[4];
+            ld_row<float, 4>(a.part + z * total, p, total, t);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += t[e];
+        }
+        const int64_t m = p / a.N, n = p % a.N;
+        if (n + 4 <= a.N) {
+            if (a.bias)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[e] += a.bias[n + e];
+            st_vec<TO, 4>((TO *)a.out + m * a.ldo + n, s);
+        } else {
+            for (int e = 0; e < 4 && p + e < total; ++e) {
+                const int64_t me = (p + e) / a.N, ne = (p + e) % a.N;
+                ((TO *)a.out)[me * a.ldo + ne] = (TO)(s[e] + (a.bias ? a.bias[ne] : 0.f));
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------ few rows
+// Up to 64 rows of a (single tokens): bound by the bytes of b, which no two workgroups
+// share.  A workgroup owns 16 rows of b; its 8 waves split the contraction (and, where
+// that leaves the chip empty, so does the grid), read b from memory straight into the
+// matrix cores' operands (a lane 32 consecutive bytes of a row, 128 bytes a row and
+// instruction), and add their tiles through LDS in the waves' order.
+// QUANT: a is bf16 or fp32 and is quantised on the way (its blocks' 128 values are in 4
+// lanes), which saves the quantiser's launch; every workgroup repeats it for its share.
+struct SkinnyArgs {
+    MatArgs m;
+    const void *x;
+    int64_t ldx;
+};
+
+template <int MT, typename TX, bool QUANT, typename TO>
+__global__ __launch_bounds__(512) void k_block_matmul_few(SkinnyArgs s) {
+    const MatArgs &a = s.m;
+    constexpr int WAVES = 8;
+    __shared__ f32x4 red[WAVES - 1][MT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int q = lane >> 4, i16 = lane & 15;
+    const int64_t n = (int64_t)blockIdx.x * 16 + i16, nc = n < a.N ? n : a.N - 1;
+    const uint8_t *brow = a.b + nc * a.ldb, *sbrow = a.sb + (nc >> a.shb) * a.lsb;
+    const int kb0 = blockIdx.y * a.kper, kb1 = kb0 + a.kper < a.ksteps ? kb0 + a.kper : a.ksteps;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // 32 bytes k .. k+31 of a row of codes, zeros from K on
+    auto codes32 = [&](const uint8_t *row, int64_t k) {
+        i32x8 f;
+        if (k + 32 <= a.K) {
+            __builtin_memcpy(&f, row + k, 32);
+        } else {
+#pragma unroll
+            for (int w = 0; w < 8; ++w) {
+                uint32_t v = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (k + 4 * w + j < a.K) v |= (uint32_t)row[k + 4 * w + j] << (8 * j);
+                f[w] = (int)v;
+            }
+        }
+        return f;
+    };
+    constexpr int U = MT <= 2 ? 4 : 2;  // blocks in flight
+    for (int kb = kb0 + wave; kb < kb1; kb += WAVES * U) {
+        i32x8 fb[U];
+        uint32_t sb[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k1 = kb + u * WAVES, kc = k1 < kb1 ? k1 : kb;
+            fb[u] = codes32(brow, (int64_t)kc * BLK + 32 * q);
+            sb[u] = sbrow[kc];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k1 = kb + u * WAVES;
+            if (k1 >= kb1) break;
+            const int64_t k = (int64_t)k1 * BLK + 32 * q;
+            const auto wb = Operand<TO>::of(fb[u], sb[u]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int64_t m = 16 * i + i16, mc = m < a.M ? m : a.M - 1;
+                i32x8 fa;
+                uint32_t sa;
+                if constexpr (QUANT) {
+                    const TX *row = (const TX *)s.x + mc * s.ldx;
+                    float v[4][8], amax = 0.f;
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        ld_row<TX, 8>(row, k + 8 * p, a.K, v[p]);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(v[p][j]));
+                    }
+                    amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
+                    amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+                    sa = (uint32_t)scale_byte(amax);
+                    const float inv = inv_scale((int)sa);
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        fa[2 * p] = (int)codes4(v[p][0] * inv, v[p][1] * inv, v[p][2] * inv, v[p][3] * inv);
+                        fa[2 * p + 1] = (int)codes4(v[p][4] * inv, v[p][5] * inv, v[p][6] * inv, v[p][7] * inv);
+                    }
+                } else {
+                    fa = codes32(a.a + mc * a.lda, k);
+                    sa = a.sa[(mc >> a.sha) * a.lsa + k1];
+                }
+                acc[i] = block_product(wb, Operand<TO>::of(fa, sa), acc[i]);
+            }
+        }
+    }
+    if (wave > 0) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) red[wave - 1][i][lane] = acc[i];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    const int64_t n4 = (int64_t)blockIdx.x * 16 + 4 * q;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int w = 0; w < WAVES - 1; ++w) acc[i] += red[w][i][lane];
+        const int64_t m = 16 * i + i16;
+        if (m >= a.M || n4 >= a.N) continue;
+        if (a.part) {
+            st_out4<float>(a.part + ((int64_t)blockIdx.y * a.M + m) * a.N + n4, acc[i], a.N - n4);
+        } else {
+            if (a.bias)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][e] += n4 + e < a.N ? a.bias[n4 + e] : 0.f;
+            st_out4<TO>((TO *)a.out + m * a.ldo + n4, acc[i], a.N - n4);
+        }
+    }
+}
+
+}  // namespace race

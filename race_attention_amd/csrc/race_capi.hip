@@ -15,12 +15,12 @@
 
 #include "../../include/race_attention.h"
 #include "prefix_mean.hip"
+#include "race_error.h"
 #include "race_kernels.hip"
 
 namespace race {
-namespace {
 
-thread_local std::string g_err;
+static thread_local std::string g_err;
 
 int fail(int code, const char *fmt, ...) {
     char buf[512];
@@ -36,6 +36,14 @@ int ok() {
     g_err.clear();
     return RACE_OK;
 }
+
+int launched(const char *what) {
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return fail(RACE_E_LAUNCH, "%s: %s", what, hipGetErrorString(e));
+    return ok();
+}
+
+namespace {
 
 // Workgroups per forward phase of long sequences (256 CUs x 8: several rounds
 // of whole segments even out), and the tiles per segment from which that many
@@ -404,12 +412,6 @@ Args base_args(const race_desc *d, const Plan &p, const float *planes) {
     a.nslice = p.nslice;
     a.Spad = p.Spad;
     return a;
-}
-
-int launched(const char *what) {
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return fail(RACE_E_LAUNCH, "%s: %s", what, hipGetErrorString(e));
-    return ok();
 }
 
 bool run_phase(const race_desc *d, int ph) { return d->phases == 0 || (d->phases & ph); }

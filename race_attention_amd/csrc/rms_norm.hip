@@ -1,0 +1,254 @@
+// rms_norm.hip -- gfx950 kernels of the root-mean-square norm with the residual's
+// addition, its backward pass, and its output in 8-bit blocks.
+//
+//   h = x + residual,  rstd = 1 / sqrt(mean(h^2) + eps),  y = h rstd w
+//   g = dy w,  dh = rstd (g - h rstd^2 mean(g h)) + dh_out,  dx = dresidual = dh,
+//   dw = sum over rows of dy h rstd
+//
+// h is rounded once, to the residual's type, where it is stored; y normalises the
+// unrounded sum.  The backward forms the same sum from x and the residual, or reads h
+// where it is fp32 (a bf16 h is 2^-9 off, which dw, a long fp32 sum, would show).
+//
+// Bound by memory: every array is read or written once.  A row is held in registers by
+// one wave (up to 1024 columns, four rows a workgroup, so that no barrier is needed and
+// a decode batch of a few rows still starts as many workgroups) or by a workgroup of
+// 256 threads (up to 16384 columns); longer rows are read twice.  Vectors start at
+// any address (an odd row length shifts every row).
+#include "layers.h"
+
+namespace race {
+
+struct NormArgs {
+    const void *x, *r, *dy, *dh;
+    const float *w;
+    const float *rstd_in;
+    void *y, *h, *dx, *dr;
+    uint8_t *scale;
+    float *rstd, *dw_part;
+    int64_t rows, D;
+    int64_t xs, rs, ys, hs, dys, dhs, dxs, drs, ss;  // row strides, elements
+    float eps;
+};
+
+constexpr int NORM_THREADS = 256;
+
+// Sum over the L threads of a row (L = 64: a wave; 256: the workgroup).
+template <int L> __device__ __forceinline__ float row_total(float x, float *part) {
+    x = lanes<64>(x, Add{});
+    if constexpr (L > 64) {
+        const int w = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) part[w] = x;
+        __syncthreads();
+        x = (part[0] + part[1]) + (part[2] + part[3]);
+        __syncthreads();
+    }
+    return x;
+}
+
+// L threads a row, NV vectors of V elements each; NV = 0: any row length, read twice.
+// CODES: y in 8-bit blocks of 128 columns.
+template <typename TX, typename TR, int V, int NV, int L, bool CODES>
+__global__ __launch_bounds__(NORM_THREADS) void k_rms_norm(NormArgs a) {
+    constexpr int RPB = NORM_THREADS / L;
+    __shared__ float part[4];
+    const int t = threadIdx.x % L;
+    const float inv_d = 1.f / (float)a.D;
+    const int nv = NV ? NV : (int)((a.D + V * L - 1) / (V * L));
+    for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / L; row < a.rows; row += (int64_t)gridDim.x * RPB) {
+        const TX *x = (const TX *)a.x + row * a.xs;
+        const TR *r = a.r ? (const TR *)a.r + row * a.rs : nullptr;
+        auto load = [&](int i, float(&v)[V]) {
+            const int64_t c = ((int64_t)i * L + t) * V;
+            ld_row<TX, V>(x, c, a.D, v);
+            if (r) {
+                float u[V];
+                ld_row<TR, V>(r, c, a.D, u);
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[j] += u[j];
+            }
+        };
+        float v[NV ? NV : 1][V], sq = 0.f;
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) load(i, v[i]);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < V; ++j) sq += v[i][j] * v[i][j];
+        } else {
+            for (int i = 0; i < nv; ++i) {
+                load(i, v[0]);
+#pragma unroll
+                for (int j = 0; j < V; ++j) sq += v[0][j] * v[0][j];
+            }
+        }
+        const float rstd = 1.f / sqrtf(row_total<L>(sq, part) * inv_d + a.eps);
+        if (a.rstd && t == 0) a.rstd[row] = rstd;
+        auto store = [&](int i, float(&v)[V]) {
+            const int64_t c = ((int64_t)i * L + t) * V;
+            if (r) st_row<TR, V>((TR *)a.h + row * a.hs, c, a.D, v);
+            float w[V];
+            ld_row<float, V>(a.w, c, a.D, w);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = v[j] * rstd * w[j];
+            if constexpr (CODES) {
+                float amax = 0.f;
+#pragma unroll
+                for (int j = 0; j < V; ++j) amax = fmaxf(amax, finite_abs(v[j]));
+                const int b = scale_byte(lanes<BLK / V>(amax, Max{}));
+                st_codes<V>((uint8_t *)a.y + row * a.ys, c, a.D, v, inv_scale(b));
+                if (c % BLK == 0 && c < a.D) a.scale[row * a.ss + c / BLK] = (uint8_t)b;
+            } else {
+                st_row<TX, V>((TX *)a.y + row * a.ys, c, a.D, v);
+            }
+        };
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) store(i, v[i]);
+        } else {
+            for (int i = 0; i < nv; ++i) {
+                load(i, v[0]);
+                store(i, v[0]);
+            }
+        }
+    }
+}
+
+// Backward.  A workgroup walks rows and keeps its part of dw in registers (NV = 0: in
+// its row of dw_part): dw_part[workgroup][D], added by k_column_sum in a fixed order.
+// The sum is x + r, or r alone where x is NULL.
+template <typename TX, typename TR, int V, int NV, int L>
+__global__ __launch_bounds__(NORM_THREADS) void k_rms_norm_bwd(NormArgs a) {
+    constexpr int RPB = NORM_THREADS / L;
+    __shared__ float part[4];
+    const int t = threadIdx.x % L;
+    const float inv_d = 1.f / (float)a.D;
+    const int nv = NV ? NV : (int)((a.D + V * L - 1) / (V * L));
+    float dw[NV ? NV : 1][V];
+#pragma unroll
+    for (int i = 0; i < (NV ? NV : 1); ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) dw[i][j] = 0.f;
+    float *out = a.dw_part + blockIdx.x * a.D;
+    if constexpr (NV == 0) {
+        for (int64_t c = threadIdx.x; c < a.D; c += NORM_THREADS) out[c] = 0.f;
+        __syncthreads();
+    }
+    for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / L; row < a.rows; row += (int64_t)gridDim.x * RPB) {
+        const TX *xp = a.x ? (const TX *)a.x + row * a.xs : nullptr;
+        const TR *rp = (const TR *)a.r + row * a.rs;
+        const TX *dyp = (const TX *)a.dy + row * a.dys;
+        const float rstd = a.rstd_in[row];
+        auto load = [&](int i, float(&h)[V], float(&dy)[V]) {
+            const int64_t c = ((int64_t)i * L + t) * V;
+            ld_row<TR, V>(rp, c, a.D, h);
+            ld_row<TX, V>(dyp, c, a.D, dy);
+            if (xp) {
+                float u[V];
+                ld_row<TX, V>(xp, c, a.D, u);
+#pragma unroll
+                for (int j = 0; j < V; ++j) h[j] += u[j];
+            }
+        };
+        float h[NV ? NV : 1][V], dy[NV ? NV : 1][V], gh = 0.f;
+        auto dot = [&](int i, const float(&h)[V], const float(&dy)[V]) {
+            float w[V];
+            ld_row<float, V>(a.w, ((int64_t)i * L + t) * V, a.D, w);
+#pragma unroll
+            for (int j = 0; j < V; ++j) gh += dy[j] * w[j] * h[j];
+        };
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) load(i, h[i], dy[i]);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) dot(i, h[i], dy[i]);
+        } else {
+            for (int i = 0; i < nv; ++i) {
+                load(i, h[0], dy[0]);
+                dot(i, h[0], dy[0]);
+            }
+        }
+        const float k = row_total<L>(gh, part) * inv_d * rstd * rstd;
+        auto finish = [&](int i, const float(&h)[V], const float(&dy)[V], float(&acc)[V]) {
+            const int64_t c = ((int64_t)i * L + t) * V;
+            float w[V], d[V];
+            ld_row<float, V>(a.w, c, a.D, w);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                acc[j] += dy[j] * (h[j] * rstd);
+                d[j] = rstd * (dy[j] * w[j] - h[j] * k);
+            }
+            if (a.dh) {
+                float u[V];
+                ld_row<TR, V>((const TR *)a.dh + row * a.dhs, c, a.D, u);
+#pragma unroll
+                for (int j = 0; j < V; ++j) d[j] += u[j];
+            }
+            if (a.dx) st_row<TX, V>((TX *)a.dx + row * a.dxs, c, a.D, d);
+            if (a.dr) st_row<TR, V>((TR *)a.dr + row * a.drs, c, a.D, d);
+        };
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) finish(i, h[i], dy[i], dw[i]);
+        } else {
+            for (int i = 0; i < nv; ++i) {
+                const int64_t c = ((int64_t)i * L + t) * V;
+                load(i, h[0], dy[0]);
+                ld_row<float, V>(out, c, a.D, dw[0]);
+                finish(i, h[0], dy[0], dw[0]);
+                st_row<float, V>(out, c, a.D, dw[0]);
+            }
+        }
+    }
+    if constexpr (NV > 0) {
+        if constexpr (RPB > 1) {
+            // the four rows' waves: added through LDS, wave by wave
+            __shared__ float acc[NV * V * L];
+            for (int w = 0; w < RPB; ++w) {
+                if (threadIdx.x / L == w) {
+#pragma unroll
+                    for (int i = 0; i < NV; ++i)
+#pragma unroll
+                        for (int j = 0; j < V; ++j) {
+                            float &s = acc[(i * V + j) * L + t];
+                            s = w ? s + dw[i][j] : dw[i][j];
+                        }
+                }
+                __syncthreads();
+            }
+            for (int i = 0; i < NV; ++i)
+                for (int jr = threadIdx.x / L; jr < V; jr += RPB) {
+                    const int64_t c = ((int64_t)i * L + t) * V + jr;
+                    if (c < a.D) out[c] = acc[(i * V + jr) * L + t];
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) st_row<float, V>(out, ((int64_t)i * L + t) * V, a.D, dw[i]);
+        }
+    }
+}
+
+// out[c] = sum over p < P of part[p][c], in a fixed order: 16 threads a column take every
+// 16th row, and their sums are added in a tree.  (fp32: at most P / 16 terms in a chain.)
+constexpr int CS_COLS = 16;
+template <typename TO>
+__global__ __launch_bounds__(256) void k_column_sum(const float *__restrict__ part, TO *__restrict__ out, int P,
+                                                    int64_t C) {
+    __shared__ float s[16][CS_COLS + 1];
+    const int cl = threadIdx.x % CS_COLS, pr = threadIdx.x / CS_COLS;
+    const int64_t c = (int64_t)blockIdx.x * CS_COLS + cl;
+    float x = 0.f;
+    if (c < C) {
+#pragma unroll 8
+        for (int p = pr; p < P; p += 16) x += part[(int64_t)p * C + c];
+    }
+    s[pr][cl] = x;
+    __syncthreads();
+    for (int n = 8; n > 0; n >>= 1) {
+        if (pr < n) s[pr][cl] += s[pr + n][cl];
+        __syncthreads();
+    }
+    if (pr == 0 && c < C) out[c] = (TO)s[0][cl];
+}
+
+}  // namespace race
