@@ -5,14 +5,14 @@ token and position embeddings, cfg["n_layers"] causal RACEBlocks
 (race_attention_amd.race.RACEBlock, misc/race.py:176-206), final LayerNorm
 and the vocabulary head.  cfg keys as the reference's GPT_CONFIG_124M:
 vocab_size, context_length, emb_dim, n_heads, n_layers, drop_rate, qkv_bias,
-K, L, M.
+K, L, M; optional norm and linear (RACEBlock).
 """
 from __future__ import annotations
 
 import torch
 from torch import nn
 
-from .race import RACEBlock
+from .race import RACEBlock, norm_of
 
 
 class LMModel(nn.Module):
@@ -23,7 +23,8 @@ class LMModel(nn.Module):
         self.tok_emb = nn.Embedding(cfg["vocab_size"], cfg["emb_dim"])
         self.pos_emb = nn.Embedding(cfg["context_length"], cfg["emb_dim"])
         self.drop_emb = nn.Dropout(cfg["drop_rate"])
-        self.final_norm = nn.LayerNorm(cfg["emb_dim"])
+        self.final_norm = norm_of(cfg, cfg["emb_dim"])
+        self.fused = cfg.get("norm", "layer") == "rms"
         self.out_head = nn.Linear(cfg["emb_dim"], cfg["vocab_size"], bias=False)
         self.blocks = nn.Sequential(*[RACEBlock(cfg, device) for _ in range(cfg["n_layers"])])
 
@@ -31,5 +32,9 @@ class LMModel(nn.Module):
         B, T = x.shape
         pos = torch.arange(T, device=x.device).unsqueeze(0)
         x = self.drop_emb(self.tok_emb(x) + self.pos_emb(pos))
-        x = self.blocks(x)
-        return self.out_head(self.final_norm(x))
+        if self.fused:  # each block's last addition is made by the next norm
+            branch, h = self.blocks((x, None))
+            x = self.final_norm(branch) if h is None else self.final_norm(branch, h)[0]
+        else:
+            x = self.final_norm(self.blocks(x))
+        return self.out_head(x)

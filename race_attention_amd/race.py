@@ -85,14 +85,15 @@ class RACEAttention(nn.Module):
     same inputs and sketch, so they are computed once (their mean equals each
     of them)."""
 
-    def __init__(self, d, h, K, L, M, drop=0.1, qkv_bias=False, device='cpu', reference_head_merge=True):
+    def __init__(self, d, h, K, L, M, drop=0.1, qkv_bias=False, device='cpu', reference_head_merge=True,
+                 linear=nn.Linear):
         super().__init__()
         assert d % h == 0
         self.h, self.d_k, self.M = h, d // h, M
-        self.q = nn.Linear(d, d, bias=qkv_bias)
-        self.k = nn.Linear(d, d, bias=qkv_bias)
-        self.v = nn.Linear(d, d, bias=qkv_bias)
-        self.o = nn.Linear(d, d)
+        self.q = linear(d, d, bias=qkv_bias)
+        self.k = linear(d, d, bias=qkv_bias)
+        self.v = linear(d, d, bias=qkv_bias)
+        self.o = linear(d, d)
         self.drop = nn.Dropout(drop)
         self.ace = BatchedACE(self.d_k, K, L, M, device=device)
         self.reference_head_merge = reference_head_merge
@@ -113,25 +114,75 @@ class RACEAttention(nn.Module):
         return self.drop(self.o(out))
 
 
-class RACEBlock(nn.Module):
-    """Pre-norm transformer block with causal RACE attention (misc/race.py:176-206).
-    cfg keys: emb_dim, n_heads, K, L, M, drop_rate, qkv_bias."""
+def linear_of(cfg):
+    """The class of a block's linear layers: cfg["linear"] "torch" (the default, as the
+    reference) or "fp8" (race_attention_amd.fp8.Linear)."""
+    kind = cfg.get("linear", "torch")
+    if kind == "torch":
+        return nn.Linear
+    if kind == "fp8":
+        from .fp8 import Linear
+        return Linear
+    raise ValueError(f"cfg['linear'] is 'torch' or 'fp8', not {kind!r}")
 
-    def __init__(self, cfg, device='cpu'):
-        super().__init__()
-        self.att = RACEAttention(d=cfg["emb_dim"], h=cfg["n_heads"], K=cfg["K"], L=cfg["L"], M=cfg["M"],
-                                 drop=cfg["drop_rate"], qkv_bias=cfg["qkv_bias"], device=device,
-                                 reference_head_merge=cfg.get("reference_head_merge", True))
-        self.norm1 = nn.LayerNorm(cfg["emb_dim"])
-        self.norm2 = nn.LayerNorm(cfg["emb_dim"])
-        self.ff = nn.Sequential(nn.Linear(cfg["emb_dim"], 4 * cfg["emb_dim"]), nn.GELU(),
-                                nn.Linear(4 * cfg["emb_dim"], cfg["emb_dim"]))
-        self.drop = nn.Dropout(cfg["drop_rate"])
+
+def norm_of(cfg, d):
+    """A block's norm: cfg["norm"] "layer" (the default, as the reference) or "rms"
+    (race_attention_amd.norm.RMSNorm)."""
+    kind = cfg.get("norm", "layer")
+    if kind == "layer":
+        return nn.LayerNorm(d)
+    if kind == "rms":
+        from .norm import RMSNorm
+        return RMSNorm(d)
+    raise ValueError(f"cfg['norm'] is 'layer' or 'rms', not {kind!r}")
+
+
+class PreNormBlock(nn.Module):
+    """x + drop(att(norm1(x))), then the same with ff and norm2: the forward of the
+    reference's blocks (misc/race.py:194-206, misc/vit.py:1056-1068).
+
+    With root-mean-square norms the additions of the residual are the norms' own, and a
+    tuple (branch, residual or None) in place of x gives one: the last addition of a block
+    is then made by the next one's norm (sum_of makes it without one)."""
+
+    def init_norms(self, cfg, d):
+        self.norm1, self.norm2 = norm_of(cfg, d), norm_of(cfg, d)
+        self.fused = cfg.get("norm", "layer") == "rms"
 
     def forward(self, x):
+        if self.fused:
+            branch, h = x if isinstance(x, tuple) else (x, None)
+            y, h = (self.norm1(branch), branch) if h is None else self.norm1(branch, h)
+            y, h = self.norm2(self.drop(self.att(y)), h)
+            y = self.drop(self.ff(y))
+            return (y, h) if isinstance(x, tuple) else sum_of((y, h))
         h = x
         x = self.att(self.norm1(x))
         x = self.drop(x) + h
         h = x
         x = self.ff(self.norm2(x))
         return self.drop(x) + h
+
+
+def sum_of(x):
+    """The tensor that a tuple (branch, residual or None) stands for."""
+    branch, h = x
+    return branch if h is None else branch + h
+
+
+class RACEBlock(PreNormBlock):
+    """Pre-norm transformer block with causal RACE attention (misc/race.py:176-206).
+    cfg keys: emb_dim, n_heads, K, L, M, drop_rate, qkv_bias; optional norm ("layer" or "rms")
+    and linear ("torch" or "fp8")."""
+
+    def __init__(self, cfg, device='cpu'):
+        super().__init__()
+        linear = linear_of(cfg)
+        self.att = RACEAttention(d=cfg["emb_dim"], h=cfg["n_heads"], K=cfg["K"], L=cfg["L"], M=cfg["M"],
+                                 drop=cfg["drop_rate"], qkv_bias=cfg["qkv_bias"], device=device,
+                                 reference_head_merge=cfg.get("reference_head_merge", True), linear=linear)
+        self.init_norms(cfg, cfg["emb_dim"])
+        self.ff = nn.Sequential(linear(cfg["emb_dim"], 4 * cfg["emb_dim"]), nn.GELU(),
+                                linear(4 * cfg["emb_dim"], cfg["emb_dim"]))
+        self.drop = nn.Dropout(cfg["drop_rate"])

@@ -15,7 +15,7 @@ import torch
 from torch import nn
 
 from .functional import LogitTemp, race_attention, race_attention_ex
-from .race import _corner_protos, merge_heads, planes_from_T
+from .race import PreNormBlock, _corner_protos, linear_of, merge_heads, norm_of, planes_from_T, sum_of
 
 
 class BatchedACE(nn.Module):
@@ -70,7 +70,7 @@ class RACEAttention(nn.Module):
     """Multi-head non-causal RACE attention (misc/vit.py:994-1039)."""
 
     def __init__(self, d_in, d_out, dropout, num_heads, L, K, N_M, qkv_bias=False, device='cpu',
-                 reference_head_merge=True):
+                 reference_head_merge=True, linear=nn.Linear):
         super().__init__()
         assert d_in % num_heads == 0
         self.H = num_heads
@@ -78,10 +78,10 @@ class RACEAttention(nn.Module):
         self.M = N_M
         self.L = L
         self.P = K
-        self.q_proj = nn.Linear(d_in, d_in, bias=qkv_bias)
-        self.k_proj = nn.Linear(d_in, d_in, bias=qkv_bias)
-        self.v_proj = nn.Linear(d_in, d_in, bias=qkv_bias)
-        self.out = nn.Linear(d_in, d_out)
+        self.q_proj = linear(d_in, d_in, bias=qkv_bias)
+        self.k_proj = linear(d_in, d_in, bias=qkv_bias)
+        self.v_proj = linear(d_in, d_in, bias=qkv_bias)
+        self.out = linear(d_in, d_out)
         self.drop = nn.Dropout(dropout)
         self.ace = BatchedACE(self.d_k, K, L, N_M, device=device)
         self.reference_head_merge = reference_head_merge
@@ -123,29 +123,22 @@ class RACEAttentionWithDenom(RACEAttention):
         return self.drop(self.out(out)), d_race_token
 
 
-class RACEBlock(nn.Module):
+class RACEBlock(PreNormBlock):
     """Pre-norm encoder block with non-causal RACE attention (misc/vit.py:1040-1068).
-    cfg keys: embed_dim, drop_rate, num_heads, qkv_bias, L, K, M."""
+    cfg keys: embed_dim, drop_rate, num_heads, qkv_bias, L, K, M; optional norm ("layer" or
+    "rms") and linear ("torch" or "fp8")."""
 
     def __init__(self, cfg, device='cpu'):
         super().__init__()
+        linear = linear_of(cfg)
         self.att = RACEAttention(d_in=cfg["embed_dim"], d_out=cfg["embed_dim"], dropout=cfg["drop_rate"],
                                  num_heads=cfg["num_heads"], qkv_bias=cfg["qkv_bias"], L=cfg["L"], K=cfg["K"],
                                  N_M=cfg["M"], device=device,
-                                 reference_head_merge=cfg.get("reference_head_merge", True))
-        self.norm1 = nn.LayerNorm(cfg["embed_dim"])
-        self.norm2 = nn.LayerNorm(cfg["embed_dim"])
-        self.ff = nn.Sequential(nn.Linear(cfg["embed_dim"], 4 * cfg["embed_dim"]), nn.GELU(),
-                                nn.Linear(4 * cfg["embed_dim"], cfg["embed_dim"]))
+                                 reference_head_merge=cfg.get("reference_head_merge", True), linear=linear)
+        self.init_norms(cfg, cfg["embed_dim"])
+        self.ff = nn.Sequential(linear(cfg["embed_dim"], 4 * cfg["embed_dim"]), nn.GELU(),
+                                linear(4 * cfg["embed_dim"], cfg["embed_dim"]))
         self.drop = nn.Dropout(cfg["drop_rate"])
-
-    def forward(self, x):
-        h = x
-        x = self.att(self.norm1(x))
-        x = self.drop(x) + h
-        h = x
-        x = self.ff(self.norm2(x))
-        return self.drop(x) + h
 
 
 class PatchEmbedding(nn.Module):
@@ -165,7 +158,8 @@ class VisionTransformer(nn.Module):
     patch embedding, CLS token, learned positions, cfg["transformer_units"]
     RACEBlocks, LayerNorm + Linear head on the CLS token.  cfg keys as the
     reference's VISION_CONFIG: img_size, patch_size, num_channels, embed_dim,
-    num_heads, transformer_units, drop_rate, qkv_bias, K, L, M, num_classes."""
+    num_heads, transformer_units, drop_rate, qkv_bias, K, L, M, num_classes; optional
+    norm and linear (RACEBlock)."""
 
     def __init__(self, cfg, attn_type="race", device='cpu'):
         super().__init__()
@@ -180,13 +174,15 @@ class VisionTransformer(nn.Module):
         nn.init.trunc_normal_(self.cls_token, std=0.02)
         nn.init.trunc_normal_(self.pos_embed, std=0.02)
         self.transformer_layers = nn.Sequential(*[RACEBlock(cfg, device) for _ in range(cfg["transformer_units"])])
-        self.mlp_head = nn.Sequential(nn.LayerNorm(d), nn.Linear(d, cfg["num_classes"]))
+        self.fused = cfg.get("norm", "layer") == "rms"
+        self.mlp_head = nn.Sequential(norm_of(cfg, d), nn.Linear(d, cfg["num_classes"]))
 
     def forward(self, x):
         x = self.patch_embedding(x)
         B = x.shape[0]
         x = torch.cat([self.cls_token.expand(B, -1, -1), x], dim=1)
         x = x + self.pos_embed[:, :x.size(1), :]
-        x = self.transformer_layers(x)
+        # root-mean-square norms: each block's last addition is made by the next one's norm
+        x = sum_of(self.transformer_layers((x, None))) if self.fused else self.transformer_layers(x)
         return self.mlp_head(x[:, 0])
 
