@@ -14,6 +14,15 @@ DTYPES = {torch.bfloat16: _lib.RACE_DTYPE_BF16, torch.float32: _lib.RACE_DTYPE_F
 _SAME = contextlib.nullcontext()
 
 
+def native(x, name, *args):
+    """The C++ call of that name (csrc/layers_torch.cpp) with these arguments, or None where it does
+    not take them: the Python path makes the call then, or raises."""
+    if not (torch.is_tensor(x) and x.is_cuda):
+        return None
+    mod = _lib.calls()
+    return None if mod is None else getattr(mod, name)(*args)
+
+
 def ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 

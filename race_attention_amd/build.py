@@ -5,7 +5,7 @@ The library is two translation units compiled side by side with hipcc for gfx950
 only: csrc/race_capi.hip (the attention operators; it includes their kernel sources)
 and csrc/layers_capi.hip (the operators around them, likewise).  Packed-fp32 instruction
 selection is disabled (-packed-fp32-ops) for all device code.  The autograd
-calls (csrc/race_torch.cpp) are host code against torch's C++ API.
+calls (csrc/race_torch.cpp, csrc/layers_torch.cpp) are host code against torch's C++ API.
 """
 import os
 import subprocess
@@ -16,7 +16,7 @@ import tempfile
 HERE = os.path.dirname(os.path.abspath(__file__))
 SRCS = [os.path.join(HERE, "csrc", name) for name in ("race_capi.hip", "layers_capi.hip")]
 OUT = os.path.join(HERE, "librace_attention.so")
-TORCH_SRC = os.path.join(HERE, "csrc", "race_torch.cpp")
+TORCH_SRCS = [os.path.join(HERE, "csrc", name) for name in ("race_torch.cpp", "layers_torch.cpp")]
 TORCH_OUT = os.path.join(HERE, "_race_torch.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
@@ -41,7 +41,7 @@ def _torch_cmd(out: str):
            sysconfig.get_paths()["include"], "/opt/rocm/include"]
     return (["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__=1",
              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + ["-I" + i for i in inc] +
-            [TORCH_SRC, "-o", out, "-L" + os.path.join(root, "lib")] +
+            TORCH_SRCS + ["-o", out, "-L" + os.path.join(root, "lib")] +
             ["-l" + x for x in ("torch", "torch_cpu", "torch_hip", "c10", "c10_hip", "torch_python")])
 
 

@@ -15,24 +15,11 @@
 // (mismatched shapes, CPU tensors, tensor subclasses, functorch transforms,
 // tracing, an active dispatch mode, a status other than RACE_OK) they return None and the caller takes the
 // Python path, whose errors and conversions are then what they always were.
-#include <dlfcn.h>
-#include <torch/extension.h>
+#include "race_torch.h"
 
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/hip/HIPFunctions.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-
-#include <string>
-
-#include "../../include/race_attention.h"
+PyObject *race_error = nullptr;
 
 namespace {
-
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
 
 // ------------------------------------------------------------ the operator library
 #define RACE_FNS(X)                                                                                              \
@@ -46,7 +33,6 @@ struct Lib {
     RACE_FNS(X)
 #undef X
 } lib;
-PyObject *race_error = nullptr;  // _lib.RaceError
 
 // The library that ctypes loaded (the same file: the same handle).
 void bind(const std::string &path, py::object error) {
@@ -59,33 +45,13 @@ void bind(const std::string &path, py::object error) {
     RACE_FNS(X)
 #undef X
     lib = l;
+    bind_layers(h, path);
     race_error = error.release().ptr();
 }
 
-// A call that these functions do not take, or whose status is an error.
-struct NotTaken {};
-
-[[noreturn]] void raise_status(const char *what, int rc) {
-    const std::string msg = std::string(what) + " failed (" + std::to_string(rc) + "): " + lib.race_last_error();
-    py::gil_scoped_acquire gil;
-    PyErr_SetString(race_error, msg.c_str());
-    python_error e;
-    e.persist();
-    throw e;
-}
+[[noreturn]] void raise_status(const char *what, int rc) { raise_race_error(what, rc, lib.race_last_error()); }
 
 // ------------------------------------------------------------ arguments
-void *stream_of(const Tensor &x) { return (void *)c10::hip::getCurrentHIPStream(x.device().index()).stream(); }
-
-// a plain strided CUDA tensor of the current device: no wrapper of a transform, a mode or a subclass
-bool plain(const Tensor &x) {
-    return x.defined() && x.is_cuda() && x.layout() == at::kStrided && x.unsafeGetTensorImpl()->has_storage() &&
-           !x.unsafeGetTensorImpl()->is_python_dispatch() && !x.is_conj() && !x.is_neg() &&
-           !x._fw_grad(/*level=*/0).defined();  // forward-mode AD: refused by the Python Functions
-}
-// torch.Tensor or torch.nn.Parameter itself (THPVariable_CheckExact takes both), no other subclass
-bool is_tensor(py::handle o) { return THPVariable_CheckExact(o.ptr()); }
-
 bool aligned(const Tensor &x) {
     const int64_t es = x.element_size();
     if (x.stride(4) != 1 || reinterpret_cast<uintptr_t>(x.data_ptr()) % 16) return false;
@@ -98,9 +64,6 @@ Tensor usable(const Tensor &x) { return aligned(x) ? x : x.contiguous(); }
 void strides4(const Tensor &x, int64_t *st) {
     for (int j = 0; j < 4; ++j) st[j] = x.size(j) > 1 ? x.stride(j) : 0;
 }
-void *ptr(const Tensor &x) { return x.data_ptr(); }
-float *fptr(const Tensor &x) { return x.defined() ? static_cast<float *>(x.data_ptr()) : nullptr; }
-
 enum Kind : int64_t { F1 = 0, EX = 1, GLOBAL = 2, PROBS = 3, PADDED = 4 };
 
 // What the forward and the backward of one call share beside tensors.
@@ -137,11 +100,6 @@ void fill_desc(race_desc &d, const Cfg &c, const Tensor &q, const Tensor &k, con
     strides4(k, d.k_stride);
     strides4(v, d.v_stride);
 }
-
-Tensor bytes(size_t n, const Tensor &like) {
-    return at::empty({(int64_t)(n < 16 ? 16 : n)}, like.options().dtype(at::kByte));
-}
-Tensor fp32(at::IntArrayRef shape, const Tensor &like) { return at::empty(shape, like.options().dtype(at::kFloat)); }
 
 // The temperature a call runs with: a device copy (made now: the source may be
 // updated in place before the backward), or for a logit the pair (inv_temp,
@@ -303,8 +261,7 @@ std::optional<Tensor> given(const Tensor &x) { return x.defined() ? std::optiona
 // the logit of an fp32 temperature clamped to [lo, hi].
 py::object call(int64_t kind, py::handle hq, py::handle hk, py::handle hv, py::handle hplanes, py::handle htemp,
                 py::handle hmask, int64_t L, int64_t K, bool causal, bool want_den, double eps, double lo, double hi) {
-    if (!is_tensor(hq) || !is_tensor(hk) || !is_tensor(hv) || !is_tensor(hplanes) || torch::jit::tracer::isTracing() ||
-        c10::impl::TorchDispatchModeTLS::any_modes_set())
+    if (!is_tensor(hq) || !is_tensor(hk) || !is_tensor(hv) || !is_tensor(hplanes) || redirected())
         return py::none();
     const Tensor &q = THPVariable_Unpack(hq.ptr()), &k = THPVariable_Unpack(hk.ptr()), &v = THPVariable_Unpack(hv.ptr());
     Tensor planes = THPVariable_Unpack(hplanes.ptr()), temp, mask;
@@ -371,6 +328,7 @@ py::object call(int64_t kind, py::handle hq, py::handle hk, py::handle hv, py::h
 } // namespace
 
 PYBIND11_MODULE(_race_torch, m) {
+    add_layers(m);
     m.def("bind", &bind);
     m.def("call", &call);
     m.attr("F1") = (int64_t)F1;

@@ -23,7 +23,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._tensors import DTYPES, on_device, ptr, require_gpu, rows2d, stream
+from ._tensors import DTYPES, native, on_device, ptr, require_gpu, rows2d, stream
 
 BLOCK = 128
 _CODES = (torch.float8_e4m3fn, torch.uint8)
@@ -161,6 +161,11 @@ def _matmul(da, db, shape, bias, out_dtype, dev):
 
 def matmul(a, b, *, bias=None, out_dtype=torch.bfloat16):
     """a b^T + bias: a BlockFp8 [..., K], b BlockFp8 [N, K], bias [N] or None -> [..., N]."""
+    if out_dtype in DTYPES:
+        out = native(a.codes, "matmul", a.codes, a.scale, a.block_rows, b.codes, b.scale, b.block_rows, bias,
+                     out_dtype is torch.float32)
+        if out is not None:
+            return out
     a.check("a")
     b.check("b")
     if b.codes.dim() != 2 or a.shape[-1] != b.shape[1]:
@@ -247,6 +252,12 @@ def linear(x, weight, bias=None):
     """x [..., K] -> [..., N] in 8 bits (see module doc): weight [N, K] as a tensor
     (differentiable) or a BlockFp8 (serving).  The result has x's type, or autocast's."""
     frozen = isinstance(weight, BlockFp8)
+    if torch.is_tensor(x) and x.dtype in DTYPES:
+        fp32 = _out_dtype(x) is torch.float32
+        out = (native(x, "linear", x, weight.codes, weight.scale, weight.block_rows, bias, fp32) if frozen
+               else native(x, "linear", x, weight, None, 0, bias, fp32))
+        if out is not None:
+            return out
     w = weight.codes if frozen else weight
     require_gpu(x, w)
     if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:

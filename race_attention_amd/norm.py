@@ -19,7 +19,7 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._tensors import DTYPES, on_device, ptr, require_gpu, rows2d, stream
+from ._tensors import DTYPES, native, on_device, ptr, require_gpu, rows2d, stream
 from .fp8 import BlockFp8, _empty_blocks
 
 
@@ -130,6 +130,9 @@ class RMSNormFunction(torch.autograd.Function):
 
 def rms_norm(x, weight, *, residual=None, eps=1e-6):
     """y, or (y, h) with a residual (see module doc)."""
+    out = native(x, "rms_norm", x, weight, residual, float(eps))
+    if out is not None:
+        return out
     needs = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
                                          (residual is not None and residual.requires_grad))
     if needs:
@@ -144,6 +147,10 @@ def rms_norm_fp8(x, weight, *, residual=None, eps=1e-6):
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
                                     (residual is not None and residual.requires_grad)):
         raise RuntimeError("rms_norm_fp8 has no backward: call it under torch.no_grad(), or use rms_norm")
+    out = native(x, "rms_norm_codes", x, weight, residual, float(eps))
+    if out is not None:
+        y = BlockFp8(*out[:2])
+        return y if residual is None else (y, out[2])
     _check(x, weight, residual)
     y = _empty_blocks(x.shape, x.device)
     h = None if residual is None else torch.empty(x.shape, dtype=residual.dtype, device=x.device)

@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._tensors import DTYPES, on_device, require_gpu, stream
+from ._tensors import DTYPES, native, on_device, require_gpu, stream
 from .fp8 import _CODES, _SCALES, BLOCK, BlockFp8
 
 
@@ -57,6 +57,18 @@ def _check_tensor(i, p, g, m, v, eight, like):
             raise _bad(i, "parameter, gradient and states are contiguous")
 
 
+def _adamw_native(params, grads, ms, vs, eight, step, lr, betas, eps, weight_decay, seed):
+    """The C++ call, where it takes these arguments."""
+    scales = [[], []]
+    if eight:
+        if not all(isinstance(s, BlockFp8) for s in ms + vs):
+            return False
+        scales = [[s.scale for s in group] for group in (ms, vs)]
+        ms, vs = [s.codes for s in ms], [s.codes for s in vs]
+    return bool(native(params[0], "adamw", params, grads, ms, vs, *scales, eight, step, float(lr), float(betas[0]),
+                       float(betas[1]), float(eps), float(weight_decay), int(seed) & 0xffffffff))
+
+
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
                seed=0):
     """One AdamW step, in place, over lists of tensors of one type (parameters and gradients
@@ -74,6 +86,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
     if not params:
         return
     eight = isinstance(ms[0], BlockFp8)
+    if _adamw_native(params, grads, ms, vs, eight, step, lr, betas, eps, weight_decay, seed):
+        return
     d = _lib.AdamwDesc()
     d.lr, (d.beta_m, d.beta_v), d.eps, d.weight_decay = float(lr), map(float, betas), float(eps), float(weight_decay)
     p0, g0 = params[0], grads[0]

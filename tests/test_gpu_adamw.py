@@ -11,10 +11,21 @@ import torch
 
 import blocks_ref as ref
 from blocks_ref import U, half_step
-from race_attention_amd import optim
+from race_attention_amd import _lib, optim
 from race_attention_amd.fp8 import BlockFp8
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, params=["c++", "python"])
+def path(request, monkeypatch):
+    """Every test through the C++ calls and through the Python ones."""
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "calls", lambda: None)
+    else:
+        assert _lib.calls() is not None
+
+
 BF, F32 = torch.bfloat16, torch.float32
 HYPER = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1)
 SHAPES = [(1,), (3, 5), (127,), (128,), (129,), (1000, 3), (0,), (64, 768), (4097,), (2, 3, 4, 5), (10001,)]

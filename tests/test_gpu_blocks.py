@@ -6,9 +6,20 @@ import pytest
 import torch
 import torch.nn.functional as F
 
-from race_attention_amd import fp8, lm, norm, optim, race, vit
+from race_attention_amd import _lib, fp8, lm, norm, optim, race, vit
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, params=["c++", "python"])
+def path(request, monkeypatch):
+    """Every test through the C++ calls and through the Python ones."""
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "calls", lambda: None)
+    else:
+        assert _lib.calls() is not None
+
+
 LM = dict(vocab_size=97, context_length=80, emb_dim=128, n_heads=2, n_layers=2, drop_rate=0.0, qkv_bias=True, K=2, L=2, M=1)
 VIT = dict(img_size=12, patch_size=4, num_channels=1, embed_dim=128, num_heads=2, transformer_units=2, drop_rate=0.0,
            qkv_bias=False, K=2, L=2, M=1, num_classes=5)

@@ -14,6 +14,17 @@ from blocks_ref import U, half_step
 from race_attention_amd import _lib, fp8
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, params=["c++", "python"])
+def path(request, monkeypatch):
+    """Every test through the C++ calls and through the Python ones."""
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "calls", lambda: None)
+    else:
+        assert _lib.calls() is not None
+
+
 BF, F32 = torch.bfloat16, torch.float32
 
 

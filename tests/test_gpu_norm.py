@@ -12,10 +12,21 @@ import torch
 
 import blocks_ref as ref
 from blocks_ref import U, half_step
-from race_attention_amd import norm
+from race_attention_amd import _lib, norm
 from race_attention_amd.fp8 import BlockFp8
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, params=["c++", "python"])
+def path(request, monkeypatch):
+    """Every test through the C++ calls and through the Python ones."""
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "calls", lambda: None)
+    else:
+        assert _lib.calls() is not None
+
+
 BF, F32 = torch.bfloat16, torch.float32
 EPS = 1e-6
 
@@ -246,3 +257,10 @@ def test_streams_and_captured_graphs(dev):
         torch.cuda.synchronize()
         got = [t.clone() for t in out]
         assert all(torch.equal(a, b) for a, b in zip(got, step())), k
+
+
+def test_second_derivatives_are_refused(dev):
+    x, w = torch.randn(3, 64, device=dev, requires_grad=True), torch.ones(64, device=dev)
+    dx, = torch.autograd.grad(norm.rms_norm(x, w).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice|does not require grad"):
+        dx.sum().backward()
