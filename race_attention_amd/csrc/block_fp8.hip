@@ -188,45 +188,34 @@ struct MatArgs {
     int tm, tn;              // tiles
 };
 
-typedef __attribute__((address_space(3))) char lds_char;
-
-// Granule (16 bytes) g of row r of an LDS tile of 128-byte rows stands at g ^ swz(r).
-// A fragment is two ds_read_b128 of granules q and q + 4, q = lane / 16 (the order of k
-// inside a block is free, as long as both operands have the same): with bits 1..3 of the
-// row in the swizzle, the 16 lanes of each of its passes ({0-3, 12-15, 20-27} and so on:
-// rows 0-3, 12-15 of one granule and 4-11 of its neighbour) fall on 16 different
-// 16-byte banks.
+// LDS tiles of the tile kernels: rows of one block, 128 bytes; granule (16 bytes) g of row r
+// stands at g ^ swz(r).  v_mfma_scale_f32_32x32x64_f8f6f4 takes half a block, a lane 32 bytes of
+// one row (the order of k is free as long as both operands have the same): granules h and h + 2
+// of the half, h = lane / 32.  With this swizzle the 16 lanes of each pass of a ds_read_b128 (rows
+// 0-3, 12-15, 20-27, then the others) fall on 16 different 16-byte banks.
 __device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
 
-// Tile of R rows: direct loads from memory to LDS, 16 bytes a lane, 8 rows a wave and
-// instruction; what lies behind the matrix reads as zeros (its offset is out of the
-// buffer's range).
-template <int R, int WAVES>
-__device__ __forceinline__ void stage(const uint8_t *base, int64_t ld, int64_t rows_left, int64_t K, int kb,
-                                      char *lds, int wave, int lane) {
-    const int64_t rows = rows_left < R ? rows_left : R;
-    // whole rows below 2^31 bytes: checked by the caller
-    __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t *>(base), 0, (int)((rows - 1) * ld + K), 0x00027000);
-    const int rl = lane >> 3, g = lane & 7;
-#pragma unroll
-    for (int i = 0; i < R / 8 / WAVES; ++i) {
-        const int r0 = (i * WAVES + wave) * 8, r = r0 + rl;
-        const int64_t k = (int64_t)kb * BLK + 16 * (g ^ swz(r));
-        const int off = r < rows && k < K ? (int)(r * ld + k) : 0x7fffffff;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void *)(lds + r0 * BLK), 16,
-                                                 off, 0, 0, 0);
-    }
+// 16 bytes a lane from base + off + soff to LDS, 1 KB a wave in lane order; zeros from size on.
+// As assembly, because the compiler would let every read of LDS wait for all such loads
+// that are on their way; the kernel waits for them itself, by their number.
+// to: LDS address.
+__device__ __forceinline__ int lds_address(const void *p) {
+    return __builtin_amdgcn_readfirstlane((int)(uintptr_t)(const __attribute__((address_space(3))) char *)p);
+}
+__device__ __forceinline__ void load_lds(const uint8_t *base, int size, int to, int off, int soff) {
+    const uint64_t p = (uint64_t)base;
+    // (the same in all lanes: scalar registers)
+    const i32x4 r = {__builtin_amdgcn_readfirstlane((int)(uint32_t)p),
+                     __builtin_amdgcn_readfirstlane((int)((uint32_t)(p >> 32) & 0xffffu)),
+                     __builtin_amdgcn_readfirstlane(size), 0x00027000};
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(off), "s"(r),
+                 "s"(soff)
+                 : "memory");
 }
 
-__device__ __forceinline__ i32x8 fragment(const char *lds, int row, int q) {
-    const i32x4 lo = *(const i32x4 *)(lds + row * BLK + 16 * (q ^ swz(row)));
-    const i32x4 hi = *(const i32x4 *)(lds + row * BLK + 16 * ((q + 4) ^ swz(row)));
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
-
-// One block of a 16x16 tile: c += 2^(sa + sb) a b^T for lanes' fragments fb (rows of b: the
-// tile's rows) and fa (rows of a: its columns).
+// c += 2^(sa + sb) a b^T for lanes' fragments fb (rows of b: the tile's rows) and fa (rows of
+// a: its columns): 128 codes of a 16x16 tile, or 64 of a 32x32 one.  S: the scale's byte.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 struct Wide { bf16x8 v[4]; };  // 32 codes as bf16, their scale applied
@@ -249,19 +238,34 @@ __device__ __forceinline__ f32x4 block_product(const Wide &b, const Wide &a, f32
     for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.v[j], a.v[j], c, 0, 0, 0);
     return c;
 }
+__device__ __forceinline__ f32x16 block_product(const Wide &b, const Wide &a, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b.v[j], a.v[j], c, 0, 0, 0);
+    return c;
+}
 struct Codes { i32x8 v; uint32_t s; };
+template <int S = 0> __device__ __forceinline__ f32x16 block_product(const Codes &b, const Codes &a, f32x16 c) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b.v, a.v, c, 0, 0, S, (int)b.s, S, (int)a.s);
+}
 __device__ __forceinline__ f32x4 block_product(const Codes &b, const Codes &a, f32x4 c) {
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.v, a.v, c, 0, 0, 0, (int)b.s, 0, (int)a.s);
 }
 // a fragment as the product of an output type takes it
 template <typename TO> struct Operand {
     typedef Codes type;
-    static __device__ __forceinline__ Codes of(const i32x8 &f, uint32_t s) { return Codes{f, s}; }
+    static __device__ __forceinline__ Codes of(const i32x8 &f, uint32_t s, int byte = 0) { return Codes{f, s}; }
 };
 template <> struct Operand<float> {
     typedef Wide type;
-    static __device__ __forceinline__ Wide of(const i32x8 &f, uint32_t s) { return widen(f, s); }
+    static __device__ __forceinline__ Wide of(const i32x8 &f, uint32_t s, int byte = 0) { return widen(f, s >> (8 * byte)); }
 };
+// a step of a 32x32 tile with byte S of the scale words
+template <int S> __device__ __forceinline__ f32x16 step_product(const Codes &b, const Codes &a, f32x16 c) {
+    return block_product<S>(b, a, c);
+}
+template <int S> __device__ __forceinline__ f32x16 step_product(const Wide &b, const Wide &a, f32x16 c) {
+    return block_product(b, a, c);
+}
 
 // four scale bytes kb .. kb+3 of a row, those from n on 0 (their codes are zeros)
 __device__ __forceinline__ uint32_t scales4(const uint8_t *row, int kb, int n) {
@@ -297,80 +301,240 @@ __device__ __forceinline__ void tile_of(int id, int tm, int tn, int &im, int &in
     in = (t - b * band) / h;
 }
 
+// A workgroup of WM x WN waves computes BM x BN outputs, a wave BM/WM x BN/WN of them in
+// 32x32 tiles.  What keeps the matrix cores fed:
+//   - the blocks of the next step travel from memory to LDS without registers while a step is
+//     multiplied (two stages); whole 128-byte lines, since the L1 fetches no less;
+//   - a wave reads the fragments of the next half block while it multiplies those of this
+//     one, so that a step's one barrier waits for nothing that was just asked for;
+//   - waves of 128 x 128 outputs (4 of them, one a SIMD): every fragment is used four times.  A
+//     CU reads 128 bytes of LDS a cycle: waves of 128 x 64 would read as long as they multiply.
+// A step is one run of instructions without a branch, in which the compiler keeps to rows of tiles:
+// loads and reads are issued between matrix instructions, which hide them.  Scales are fetched 16
+// steps at a time (a row's 16 bytes; every fetch costs a line of the L1) and read from LDS step by step.
+// The outputs leave through LDS in whole rows.
 template <int BM, int BN, int WM, int WN, typename TO>
-__global__ __launch_bounds__(64 * WM * WN) void k_block_matmul(MatArgs a) {
-    constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
-    __shared__ __align__(16) char buf[2][(BM + BN) * BLK];
+__global__ __launch_bounds__(64 * WM * WN, 1) void k_block_matmul(MatArgs a) {
+    constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * BLK;
+    constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;  // loads of 1 KB, 8 rows, a wave and step
+    constexpr int SR = (BM + BN) / (64 * WAVES);             // rows whose scales a thread fetches
+    constexpr int ROW = BN / WN * (int)sizeof(TO);           // bytes of a row of a wave's outputs
+    static_assert(BM % 64 == 0 && SR >= 1, "a wave fetches scales of a or of b");
+    static_assert(WAVES % 2 == 0, "bit 3 of a load's first row is the wave's lowest");
+    static_assert(WAVES * (BM / WM) * ROW <= 2 * STAGE, "the outputs fit the stages");
+    constexpr int SG = 16;                                   // steps of a fetch of scales
+    __shared__ __align__(16) char buf[2 * STAGE];
+    __shared__ __align__(16) uint8_t sc[2][BM + BN][SG];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int wm = wave / WN, wn = wave % WN, q = lane >> 4, i16 = lane & 15;
+    const int wm = wave / WN, wn = wave % WN, h = lane >> 5, i32 = lane & 31;
     int im, in;
     tile_of(blockIdx.x, a.tm, a.tn, im, in);
     const int64_t m0 = (int64_t)im * BM, n0 = (int64_t)in * BN;
     const int kb0 = blockIdx.y * a.kper, kb1 = kb0 + a.kper < a.ksteps ? kb0 + a.kper : a.ksteps;
-    const uint8_t *abase = a.a + m0 * a.lda, *bbase = a.b + n0 * a.ldb;
-    const uint8_t *srow_a[TM], *srow_b[TN];
+    // bytes of the contraction that this workgroup takes, from kb0 * BLK on
+    const int klen = (int)((int64_t)kb1 * BLK < a.K ? (int64_t)(kb1 - kb0) * BLK : a.K - (int64_t)kb0 * BLK);
+    const int steps = kb1 - kb0;
+    const int arows = a.M - m0 < BM ? (int)(a.M - m0) : BM, brows = a.N - n0 < BN ? (int)(a.N - n0) : BN;
+    const uint8_t *abase = a.a + m0 * a.lda + (int64_t)kb0 * BLK, *bbase = a.b + n0 * a.ldb + (int64_t)kb0 * BLK;
+    const int asize = (int)((arows - 1) * a.lda) + klen, bsize = (int)((brows - 1) * a.ldb) + klen;
+    // this lane's granule in each of its loads; rows behind the matrix: out of any range, read as zeros
+    constexpr int OUT = 0x7fffffff;
+    int off[LA + LB];
+    const int g16 = 16 * ((lane & 7) ^ swz((wave & 1) * 8 + (lane >> 3)));
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const int64_t m = m0 + (wm * TM + i) * 16 + i16;
-        srow_a[i] = a.sa + ((m < a.M ? m : a.M - 1) >> a.sha) * a.lsa;
+    for (int i = 0; i < LA + LB; ++i) {
+        const bool isa = i < LA;
+        const int r = ((isa ? i : i - LA) * WAVES + wave) * 8 + (lane >> 3);
+        off[i] = r < (isa ? arows : brows) ? (int)(r * (isa ? a.lda : a.ldb)) + g16 : OUT;
     }
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const int64_t n = n0 + (wn * TN + j) * 16 + i16;
-        srow_b[j] = a.sb + ((n < a.N ? n : a.N - 1) >> a.shb) * a.lsb;
-    }
-    auto load = [&](int kb, char *to) {
-        stage<BM, WAVES>(abase, a.lda, a.M - m0, a.K, kb, to, wave, lane);
-        stage<BN, WAVES>(bbase, a.ldb, a.N - n0, a.K, kb, to + BM * BLK, wave, lane);
+    const int lds = lds_address(buf) + wave * 1024;
+    auto load = [&](int s, int i) {  // load i of step s; behind the last step nothing is read (a size of 0)
+        const bool live = s < steps;
+        const int to = lds + (s & 1) * STAGE + (i < LA ? i * WAVES * 1024 : BM * BLK + (i - LA) * WAVES * 1024);
+        load_lds(i < LA ? abase : bbase, live ? (i < LA ? asize : bsize) : 0, to, off[i], live ? s * BLK : 0);
     };
-    f32x4 acc[TM][TN];
+    auto cut = [&] {  // before the loads of the last step: what lies behind the row's last code is not read
+        if ((steps - 1) * BLK + g16 >= klen) {
+#pragma unroll
+            for (int i = 0; i < LA + LB; ++i) off[i] = OUT;
+        }
+    };
+    const uint8_t *sp[SR];
+#pragma unroll
+    for (int i = 0; i < SR; ++i) {
+        const int r = i * 64 * WAVES + (int)threadIdx.x, rb = r - BM;
+        if (r < BM) sp[i] = a.sa + ((m0 + (r < arows ? r : arows - 1)) >> a.sha) * a.lsa;
+        else sp[i] = a.sb + ((n0 + (rb < brows ? rb : brows - 1)) >> a.shb) * a.lsb;
+    }
+    i32x4 word[SR];
+    auto fetch_scales = [&](int s) {  // of steps s .. s+15; those behind the last are not used
+#pragma unroll
+        for (int i = 0; i < SR; ++i) {
+            word[i] = i32x4{0, 0, 0, 0};
+            if (s + SG <= steps) {
+                __builtin_memcpy(&word[i], sp[i] + kb0 + s, SG);
+            } else {
+                for (int j = 0; s + j < steps; ++j) word[i][j >> 2] |= (int)((uint32_t)sp[i][kb0 + s + j] << (8 * (j & 3)));
+            }
+        }
+    };
+    auto put_scales = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < SR; ++i) *(i32x4 *)sc[(s / SG) & 1][i * 64 * WAVES + threadIdx.x] = word[i];
+    };
+    uint32_t sa[TM], sb[TN], na[TM], nb[TN];  // of this step and the next
+    auto read_scales = [&](int s) {
+        const uint8_t *p = &sc[(s / SG) & 1][i32][s % SG];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) na[i] = p[(wm * TM + i) * 32 * SG];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) nb[j] = p[(BM + (wn * TN + j) * 32) * SG];
+    };
+    // fragments of half u of a stage: rows of 32, granules 4u + h and 4u + h + 2
+    const int fo = i32 * BLK + 16 * (h ^ swz(i32));
+    const int fa = wm * TM * 32 * BLK + fo, fb = (BM + wn * TN * 32) * BLK + fo;
+    auto fragment = [&](const char *tile, int at) {
+        const i32x4 lo = *(const i32x4 *)(tile + at), hi = *(const i32x4 *)(tile + (at ^ 32));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    i32x8 ca[2][TM], cb[2][TN];
+    auto read = [&](const char *stage, auto U, int k) {  // fragment k of a half: those of b, then of a
+        constexpr int u = U;
+        if (k < TN) cb[u][k] = fragment(stage + k * 32 * BLK, fb ^ (64 * u));
+        else ca[u][k - TN] = fragment(stage + (k - TN) * 32 * BLK, fa ^ (64 * u));
+    };
+    f32x16 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    uint32_t sa[TM], sb[TN];
-    load(kb0, buf[0]);
-    for (int kb = kb0; kb < kb1; ++kb) {
-        const int cur = (kb - kb0) & 1;
-        if (((kb - kb0) & 3) == 0) {
+        for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int i = 0; i < TM; ++i) sa[i] = scales4(srow_a[i], kb, a.ksteps);
-#pragma unroll
-            for (int j = 0; j < TN; ++j) sb[j] = scales4(srow_b[j], kb, a.ksteps);
-        }
-        __syncthreads();  // the tile of kb is in LDS; the other buffer's readers are done
-        if (kb + 1 < kb1) load(kb + 1, buf[cur ^ 1]);
-        const char *ta = buf[cur], *tb = ta + BM * BLK;
-        typename Operand<TO>::type fb[TN];
-#pragma unroll
-        for (int j = 0; j < TN; ++j) fb[j] = Operand<TO>::of(fragment(tb, (wn * TN + j) * 16 + i16, q), sb[j]);
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    // One half: a row of tiles at a time, and between them what `with` issues, which the
+    // matrix instructions of the row (TN of 64 cycles) hide.  The compiler keeps to the rows.
+    auto multiply = [&](auto U, auto with) {
+        constexpr int u = U;
+        typename Operand<TO>::type wb[TN];
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-            const typename Operand<TO>::type fa = Operand<TO>::of(fragment(ta, (wm * TM + i) * 16 + i16, q), sa[i]);
+            with(i);
+            if (i == 0) {
 #pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = block_product(fb[j], fa, acc[i][j]);
+                for (int j = 0; j < TN; ++j) wb[j] = Operand<TO>::of(cb[u][j], sb[j]);
+            }
+            const typename Operand<TO>::type wa = Operand<TO>::of(ca[u][i], sa[i]);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = block_product(wb[j], wa, acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
         }
+    };
+    constexpr std::integral_constant<int, 0> first{};
+    constexpr std::integral_constant<int, 1> second{};
+    constexpr int HALF = TM / 2;                             // reads go with the first rows: done by the barrier
+    constexpr int READS = (TM + TN + HALF - 1) / HALF, LOADS = (LA + LB + TM - 1) / TM;  // with each row
+    fetch_scales(0);
+    put_scales(0);
+    if (steps == 1) cut();
 #pragma unroll
-        for (int i = 0; i < TM; ++i) sa[i] >>= 8;
+    for (int i = 0; i < LA + LB; ++i) load(0, i);
+    if (steps == 2) cut();
 #pragma unroll
-        for (int j = 0; j < TN; ++j) sb[j] >>= 8;
+    for (int i = 0; i < LA + LB; ++i) load(1, i);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LA + LB) : "memory");
+#pragma unroll
+    for (int k = 0; k < TM + TN; ++k) read(buf, first, k);
+    read_scales(0);
+    for (int s = 0; s < steps;) {
+        if (s % SG == 0) {
+            if (s) put_scales(s + SG);
+            else fetch_scales(SG), put_scales(SG);
+            fetch_scales(s + 2 * SG);
+        }
+        if (s == steps - 3) cut();
+        int end = s - s % SG + SG < steps ? s - s % SG + SG : steps;
+        if (s < steps - 3 && end > steps - 3) end = steps - 3;
+#pragma clang loop unroll(disable)
+        for (; s < end; ++s) {
+            const char *cur = buf + (s & 1) * STAGE, *nxt = buf + (~s & 1) * STAGE;
+#pragma unroll
+            for (int i = 0; i < TM; ++i) sa[i] = na[i];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) sb[j] = nb[j];
+            multiply(first, [&](int i) {
+#pragma unroll
+                for (int k = i * READS; k < (i + 1) * READS && k < TM + TN; ++k) read(cur, second, k);
+            });
+            // the next step is in LDS, and every wave has read this one
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(second, [&](int i) {
+#pragma unroll
+                for (int k = i * READS; k < (i + 1) * READS && k < TM + TN; ++k) read(nxt, first, k);
+#pragma unroll
+                for (int k = i * LOADS; k < (i + 1) * LOADS && k < LA + LB; ++k) load(s + 2, k);
+                if (i == TM - 1) read_scales(s + 1);
+            });
+        }
     }
-    // lane: column i16 of the product's tile (a row of a), rows 4q .. 4q+3 (rows of b)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const int64_t n = n0 + (wn * TN + j) * 16 + 4 * q;
-        f32x4 bias = {0.f, 0.f, 0.f, 0.f};
-        if (a.bias && !a.part)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) bias[e] = n + e < a.N ? a.bias[n + e] : 0.f;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the stages are read, and no load is on its way
+    // lane: column i32 of a tile (a row of a), rows 8 e + 4 h .. + 3 (rows of b)
+    if (a.part) {
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-            const int64_t m = m0 + (wm * TM + i) * 16 + i16;
-            if (m >= a.M || n >= a.N) continue;
-            if (a.part)
-                st_out4<float>(a.part + ((int64_t)blockIdx.y * a.M + m) * a.N + n, acc[i][j], a.N - n);
-            else
-                st_out4<TO>((TO *)a.out + m * a.ldo + n, acc[i][j] + bias, a.N - n);
+            const int64_t m = m0 + (wm * TM + i) * 32 + i32, n = n0 + wn * TN * 32 + 4 * h;
+            float *row = a.part + ((int64_t)blockIdx.y * a.M + m) * a.N;
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int64_t c = n + j * 32 + 8 * e;
+                    const f32x4 v = {acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+                    if (m < a.M && c < a.N) st_out4<float>(row + c, v, a.N - c);
+                }
+        }
+        return;
+    }
+    // a wave's rows, granules swizzled by the row: 16 lanes' pieces of 16 rows in 16 banks
+    constexpr int G = ROW / 16;
+    char *mine = buf + wave * (TM * 32 * ROW);
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int c = j * 32 + 8 * e + 4 * h;
+            const int64_t n = n0 + wn * TN * 32 + c;
+            f32x4 bias = {0.f, 0.f, 0.f, 0.f};
+            if (a.bias)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) bias[k] = n + k < a.N ? a.bias[n + k] : 0.f;
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const float t[4] = {acc[i][j][4 * e] + bias[0], acc[i][j][4 * e + 1] + bias[1],
+                                    acc[i][j][4 * e + 2] + bias[2], acc[i][j][4 * e + 3] + bias[3]};
+                const int byte = c * (int)sizeof(TO), r = i * 32 + i32;
+                char *p = mine + r * ROW + 16 * ((byte / 16) ^ (r & (G - 1))) + byte % 16;
+                st_vec<TO, 4>((TO *)__builtin_assume_aligned(p, 4 * sizeof(TO)), t);
+            }
+        }
+    constexpr int RPI = 64 / G;  // rows an instruction
+    constexpr int PIECE = 16 / (int)sizeof(TO);
+    const int g = lane % G;
+    const int64_t n = n0 + wn * TN * 32 + g * PIECE;
+#pragma unroll 4
+    for (int i = 0; i < TM * 32 / RPI; ++i) {
+        const int r = i * RPI + lane / G;
+        const int64_t m = m0 + wm * TM * 32 + r;
+        const i32x4 v = *(const i32x4 *)(mine + r * ROW + 16 * (g ^ (r & (G - 1))));
+        if (m >= a.M) continue;
+        TO *p = (TO *)a.out + m * a.ldo + n;
+        if (n + PIECE <= a.N) {
+            __builtin_memcpy(p, &v, 16);
+        } else {
+            TO t[PIECE];
+            __builtin_memcpy(t, &v, 16);
+#pragma unroll
+            for (int k = 0; k < PIECE; ++k)
+                if (n + k < a.N) p[k] = t[k];
         }
     }
 }

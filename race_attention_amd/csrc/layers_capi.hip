@@ -211,7 +211,7 @@ template <typename TO> void launch_sum(const MatArgs &m, int splits, hipStream_t
 template <typename TO> void launch_tiles(const MatPlan &p, const MatArgs &m, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)p.tm * p.tn), (unsigned)p.splits);
     if constexpr (!std::is_same<TO, float>::value) {
-        if (p.bm == 256) k_block_matmul<256, 256, 2, 4, TO><<<grid, 512, 0, s>>>(m);
+        if (p.bm == 256) k_block_matmul<256, 256, 2, 2, TO><<<grid, 256, 0, s>>>(m);
     }
     if (p.bm == 128) k_block_matmul<128, 128, 2, 2, TO><<<grid, 256, 0, s>>>(m);
     if (p.splits > 1) launch_sum<TO>(m, p.splits, s);
