@@ -318,13 +318,13 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_block_matmul(MatArgs a) {
     constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, STAGE = (BM + BN) * BLK;
     constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;  // loads of 1 KB, 8 rows, a wave and step
     constexpr int SR = (BM + BN) / (64 * WAVES);             // rows whose scales a thread fetches
-    constexpr int ROW = BN / WN * (int)sizeof(TO);           // bytes of a row of a wave's outputs
+    constexpr bool SPLITS = BM == 128;                       // fp32 parts fit the stages
     static_assert(BM % 64 == 0 && SR >= 1, "a wave fetches scales of a or of b");
     static_assert(WAVES % 2 == 0, "bit 3 of a load's first row is the wave's lowest");
-    static_assert(WAVES * (BM / WM) * ROW <= 2 * STAGE, "the outputs fit the stages");
+    static_assert(BM * BN * (SPLITS ? 4 : (int)sizeof(TO)) <= 2 * STAGE, "the outputs fit the stages");
     constexpr int SG = 16;                                   // steps of a fetch of scales
     __shared__ __align__(16) char buf[2 * STAGE];
-    __shared__ __align__(16) uint8_t sc[2][BM + BN][SG];
+    __shared__ uint8_t sc[2][SG][BM + BN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN, h = lane >> 5, i32 = lane & 31;
     int im, in;
@@ -370,25 +370,30 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_block_matmul(MatArgs a) {
     auto fetch_scales = [&](int s) {  // of steps s .. s+15; those behind the last are not used
 #pragma unroll
         for (int i = 0; i < SR; ++i) {
-            word[i] = i32x4{0, 0, 0, 0};
             if (s + SG <= steps) {
                 __builtin_memcpy(&word[i], sp[i] + kb0 + s, SG);
-            } else {
-                for (int j = 0; s + j < steps; ++j) word[i][j >> 2] |= (int)((uint32_t)sp[i][kb0 + s + j] << (8 * (j & 3)));
+            } else {  // bytes, none behind the row's last: all on their way at once
+                uint8_t b[SG];
+#pragma unroll
+                for (int j = 0; j < SG; ++j) b[j] = sp[i][kb0 + (s + j < steps ? s + j : steps - 1)];
+                __builtin_memcpy(&word[i], b, SG);
             }
         }
     };
     auto put_scales = [&](int s) {
 #pragma unroll
-        for (int i = 0; i < SR; ++i) *(i32x4 *)sc[(s / SG) & 1][i * 64 * WAVES + threadIdx.x] = word[i];
+        for (int i = 0; i < SR; ++i)
+#pragma unroll
+            for (int j = 0; j < SG; ++j)
+                sc[(s / SG) & 1][j][i * 64 * WAVES + threadIdx.x] = (uint8_t)(word[i][j >> 2] >> (8 * (j & 3)));
     };
     uint32_t sa[TM], sb[TN], na[TM], nb[TN];  // of this step and the next
     auto read_scales = [&](int s) {
-        const uint8_t *p = &sc[(s / SG) & 1][i32][s % SG];
+        const uint8_t *p = &sc[(s / SG) & 1][s % SG][i32];
 #pragma unroll
-        for (int i = 0; i < TM; ++i) na[i] = p[(wm * TM + i) * 32 * SG];
+        for (int i = 0; i < TM; ++i) na[i] = p[(wm * TM + i) * 32];
 #pragma unroll
-        for (int j = 0; j < TN; ++j) nb[j] = p[(BM + (wn * TN + j) * 32) * SG];
+        for (int j = 0; j < TN; ++j) nb[j] = p[BM + (wn * TN + j) * 32];
     };
     // fragments of half u of a stage: rows of 32, granules 4u + h and 4u + h + 2
     const int fo = i32 * BLK + 16 * (h ^ swz(i32));
@@ -432,23 +437,23 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_block_matmul(MatArgs a) {
     constexpr std::integral_constant<int, 1> second{};
     constexpr int HALF = TM / 2;                             // reads go with the first rows: done by the barrier
     constexpr int READS = (TM + TN + HALF - 1) / HALF, LOADS = (LA + LB + TM - 1) / TM;  // with each row
-    fetch_scales(0);
-    put_scales(0);
     if (steps == 1) cut();
 #pragma unroll
     for (int i = 0; i < LA + LB; ++i) load(0, i);
     if (steps == 2) cut();
 #pragma unroll
     for (int i = 0; i < LA + LB; ++i) load(1, i);
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LA + LB) : "memory");
+    fetch_scales(0);
+    put_scales(0);  // (waits for the words, and so for the loads before them)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
     for (int k = 0; k < TM + TN; ++k) read(buf, first, k);
     read_scales(0);
     for (int s = 0; s < steps;) {
         if (s % SG == 0) {
-            if (s) put_scales(s + SG);
-            else fetch_scales(SG), put_scales(SG);
-            fetch_scales(s + 2 * SG);
+            if (s == 0 && SG < steps) fetch_scales(SG);
+            if (s + SG < steps) put_scales(s + SG);
+            if (s + 2 * SG < steps) fetch_scales(s + 2 * SG);
         }
         if (s == steps - 3) cut();
         int end = s - s % SG + SG < steps ? s - s % SG + SG : steps;
@@ -472,71 +477,61 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_block_matmul(MatArgs a) {
                 for (int k = i * READS; k < (i + 1) * READS && k < TM + TN; ++k) read(nxt, first, k);
 #pragma unroll
                 for (int k = i * LOADS; k < (i + 1) * LOADS && k < LA + LB; ++k) load(s + 2, k);
-                if (i == TM - 1) read_scales(s + 1);
+                if (i == HALF) read_scales(s + 1);
             });
         }
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the stages are read, and no load is on its way
-    // lane: column i32 of a tile (a row of a), rows 8 e + 4 h .. + 3 (rows of b)
-    if (a.part) {
+    // Outputs through LDS.  A lane holds column i32 of each tile (a row of a) and rows 8 e + 4 h .. + 3
+    // (rows of b).  A wave's rows have their granules swizzled by the row: 16 lanes' pieces of 16
+    // rows in 16 banks.  EO: the stored type, of out or of a part.
+    auto store = [&](auto *out, int64_t ldo, const float *bias_of) {
+        typedef std::remove_pointer_t<decltype(out)> EO;
+        constexpr int ROW = BN / WN * (int)sizeof(EO), G = ROW / 16, RPI = 64 / G, PIECE = 16 / (int)sizeof(EO);
+        char *mine = buf + wave * (TM * 32 * ROW);
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int64_t m = m0 + (wm * TM + i) * 32 + i32, n = n0 + wn * TN * 32 + 4 * h;
-            float *row = a.part + ((int64_t)blockIdx.y * a.M + m) * a.N;
+        for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int j = 0; j < TN; ++j)
+            for (int e = 0; e < 4; ++e) {
+                const int c = j * 32 + 8 * e + 4 * h;
+                const int64_t n = n0 + wn * TN * 32 + c;
+                f32x4 bias = {0.f, 0.f, 0.f, 0.f};
+                if (bias_of)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int64_t c = n + j * 32 + 8 * e;
-                    const f32x4 v = {acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
-                    if (m < a.M && c < a.N) st_out4<float>(row + c, v, a.N - c);
+                    for (int k = 0; k < 4; ++k) bias[k] = n + k < a.N ? bias_of[n + k] : 0.f;
+#pragma unroll
+                for (int i = 0; i < TM; ++i) {
+                    const float t[4] = {acc[i][j][4 * e] + bias[0], acc[i][j][4 * e + 1] + bias[1],
+                                        acc[i][j][4 * e + 2] + bias[2], acc[i][j][4 * e + 3] + bias[3]};
+                    const int byte = c * (int)sizeof(EO), r = i * 32 + i32;
+                    char *p = mine + r * ROW + 16 * ((byte / 16) ^ (r & (G - 1))) + byte % 16;
+                    st_vec<EO, 4>((EO *)__builtin_assume_aligned(p, 4 * sizeof(EO)), t);
                 }
-        }
-        return;
-    }
-    // a wave's rows, granules swizzled by the row: 16 lanes' pieces of 16 rows in 16 banks
-    constexpr int G = ROW / 16;
-    char *mine = buf + wave * (TM * 32 * ROW);
+            }
+        const int g = lane % G;
+        const int64_t n = n0 + wn * TN * 32 + g * PIECE;
+#pragma unroll 4
+        for (int i = 0; i < TM * 32 / RPI; ++i) {
+            const int r = i * RPI + lane / G;
+            const int64_t m = m0 + wm * TM * 32 + r;
+            const i32x4 v = *(const i32x4 *)(mine + r * ROW + 16 * (g ^ (r & (G - 1))));
+            if (m >= a.M) continue;
+            EO *p = out + m * ldo + n;
+            if (n + PIECE <= a.N) {
+                __builtin_memcpy(p, &v, 16);
+            } else {
+                EO t[PIECE];
+                __builtin_memcpy(t, &v, 16);
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int c = j * 32 + 8 * e + 4 * h;
-            const int64_t n = n0 + wn * TN * 32 + c;
-            f32x4 bias = {0.f, 0.f, 0.f, 0.f};
-            if (a.bias)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) bias[k] = n + k < a.N ? a.bias[n + k] : 0.f;
-#pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                const float t[4] = {acc[i][j][4 * e] + bias[0], acc[i][j][4 * e + 1] + bias[1],
-                                    acc[i][j][4 * e + 2] + bias[2], acc[i][j][4 * e + 3] + bias[3]};
-                const int byte = c * (int)sizeof(TO), r = i * 32 + i32;
-                char *p = mine + r * ROW + 16 * ((byte / 16) ^ (r & (G - 1))) + byte % 16;
-                st_vec<TO, 4>((TO *)__builtin_assume_aligned(p, 4 * sizeof(TO)), t);
+                for (int k = 0; k < PIECE; ++k)
+                    if (n + k < a.N) p[k] = t[k];
             }
         }
-    constexpr int RPI = 64 / G;  // rows an instruction
-    constexpr int PIECE = 16 / (int)sizeof(TO);
-    const int g = lane % G;
-    const int64_t n = n0 + wn * TN * 32 + g * PIECE;
-#pragma unroll 4
-    for (int i = 0; i < TM * 32 / RPI; ++i) {
-        const int r = i * RPI + lane / G;
-        const int64_t m = m0 + wm * TM * 32 + r;
-        const i32x4 v = *(const i32x4 *)(mine + r * ROW + 16 * (g ^ (r & (G - 1))));
-        if (m >= a.M) continue;
-        TO *p = (TO *)a.out + m * a.ldo + n;
-        if (n + PIECE <= a.N) {
-            __builtin_memcpy(p, &v, 16);
-        } else {
-            TO t[PIECE];
-            __builtin_memcpy(t, &v, 16);
-#pragma unroll
-            for (int k = 0; k < PIECE; ++k)
-                if (n + k < a.N) p[k] = t[k];
-        }
+    };
+    if constexpr (SPLITS) {
+        if (a.part) return store(a.part + (int64_t)blockIdx.y * a.M * a.N, a.N, nullptr);
     }
+    store((TO *)a.out, a.ldo, a.bias);
 }
 
 // The parts of a split contraction, added in order, with the bias.

@@ -186,14 +186,30 @@ int mat_plan(const race_blocks *a, const race_blocks *b, int out_dtype, MatPlan 
         const int64_t lda = p.pack_a ? p.K : a->ld, ldb = p.pack_b ? p.K : b->ld;
         if (lda >= (1 << 22) || ldb >= (1 << 22))
             return fail(RACE_E_UNSUPPORTED, "row pitch of 2^22 bytes or more (a %lld, b %lld)", (ll)lda, (ll)ldb);
-        p.bm = p.bn = 256;
-        if (out_dtype == RACE_DTYPE_F32 || ceil_div(p.M, 256) * ceil_div(p.N, 256) < kCUs) p.bm = p.bn = 128;
+        // Tiles of 256 x 256 (one workgroup a CU) feed the matrix cores better, 1.6 us a step
+        // against 2 x 1.0 us of the four times smaller work of 128 x 128 (two a CU); but no other workgroup
+        // works while one begins and ends, 12 us against 4.  128 x 128 may also split the contraction;
+        // its parts are written and read once (4 TB/s) and take a launch.  The least estimate is taken.
+        // us, 256 and 128: 8192^3 402 and 493; 4096^3 59 and 65; 50240 x 1536, K = 384, 82 and 64;
+        // 8192 x 2304, K = 768, 40 and 28.  (fp32 outputs: the bf16 operands take 128 x 128's registers.)
+        const int64_t big = ceil_div(p.M, 256) * ceil_div(p.N, 256), small = ceil_div(p.M, 128) * ceil_div(p.N, 128);
+        double best = out_dtype == RACE_DTYPE_F32 ? 1e30 : (double)ceil_div(big, kCUs) * (1.6 * p.ksteps + 12);
+        p.bm = 256;
+        for (int s = 1; s == 1 || (s <= 64 && 2 * s <= p.ksteps && (s - 1) * small < 2 * kCUs); ++s) {
+            const int64_t wgs = small * s;
+            const double step = wgs <= kCUs ? 0.65 : 1.0;
+            const double t = (double)ceil_div(wgs, 2 * kCUs) * (step * ceil_div(p.ksteps, s) + 4) +
+                             (s > 1 ? 4 + 2e-6 * s * p.M * p.N : 0.0);
+            if (t < best) {
+                best = t;
+                p.bm = 128;
+                p.splits = s;
+            }
+        }
+        p.bn = p.bm;
         p.tm = (int)ceil_div(p.M, p.bm);
         p.tn = (int)ceil_div(p.N, p.bn);
         const int64_t tiles = (int64_t)p.tm * p.tn;
-        const int64_t slots = (p.bm == 128 ? 2 : 1) * kCUs;
-        int64_t want = slots / tiles, most = ceil_div(p.ksteps, 4);
-        p.splits = (int)(want < 1 ? 1 : want < most ? want : most);
         if (tiles > (1 << 22)) return fail(RACE_E_UNSUPPORTED, "%d x %d outputs exceed one launch", p.M, p.N);
     }
     if (p.splits < 1) p.splits = 1;
