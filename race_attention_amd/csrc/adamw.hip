@@ -128,7 +128,7 @@ template <typename TP, typename TG, bool EIGHT> __global__ __launch_bounds__(ADA
                 ar = fmaxf(ar, finite_abs(root[j]));
             }
             const int bm = scale_byte(row16(am, Max{})), br = scale_byte(row16(ar, Max{}));
-            const float im = inv_scale(bm), ir = inv_scale(br);
+            const float im = scale_of(254 - bm), ir = scale_of(254 - br);  // 2^-s (bytes are at most 247)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const uint32_t h = mix32(a.place[t] + (uint32_t)(c + j) + mixed_seed);

@@ -31,19 +31,106 @@ struct QuantArgs {
     float *sums;                 // [ceil(rows / 128)][cols] column sums of 128 rows, nullable
 };
 
+// Elements of 8 columns as the quantisers hold them: bf16 as it is, in pairs, for which
+// comparing and converting take an instruction a pair, or fp32.
+template <typename T> struct Eight;
+template <> struct Eight<bf16> {
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const bf16 *row, int64_t c, int64_t n) {
+        if (c + 8 <= n) {
+            __builtin_memcpy(w, row + c, 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = 0;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    uint16_t x = 0;
+                    if (c + 2 * j + k < n) __builtin_memcpy(&x, row + c + 2 * j + k, 2);
+                    w[j] |= (uint32_t)x << (16 * k);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = 0;
+    }
+    __device__ __forceinline__ float amax() const {
+        u16x2 m = finite_abs2(w[0]);
+#pragma unroll
+        for (int j = 1; j < 4; ++j) m = __builtin_elementwise_max(m, finite_abs2(w[j]));
+        return larger(m);
+    }
+    __device__ __forceinline__ float value(int j) const {
+        return __builtin_bit_cast(float, j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+    }
+    __device__ __forceinline__ void codes(float scale, uint32_t (&q)[2]) const {
+        q[0] = codes4(w[0], w[1], scale);
+        q[1] = codes4(w[2], w[3], scale);
+    }
+    // of column j of four rows
+    static __device__ __forceinline__ uint32_t down(const Eight (&v)[8], int r, int j, float scale) {
+        const uint32_t pick = j & 1 ? 0x07060302u : 0x05040100u;  // the high or the low halves of two words
+        return codes4(__builtin_amdgcn_perm(v[r + 1].w[j / 2], v[r].w[j / 2], pick),
+                      __builtin_amdgcn_perm(v[r + 3].w[j / 2], v[r + 2].w[j / 2], pick), scale);
+    }
+    // amax of each column over 8 rows
+    static __device__ __forceinline__ void columns(const Eight (&v)[8], float (&m)[8]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            u16x2 x = finite_abs2(v[0].w[j]);
+#pragma unroll
+            for (int r = 1; r < 8; ++r) x = __builtin_elementwise_max(x, finite_abs2(v[r].w[j]));
+            m[2 * j] = __builtin_bit_cast(float, (uint32_t)x[0] << 16);
+            m[2 * j + 1] = __builtin_bit_cast(float, (uint32_t)x[1] << 16);
+        }
+    }
+};
+template <> struct Eight<float> {
+    float f[8];
+    __device__ __forceinline__ void load(const float *row, int64_t c, int64_t n) { ld_row<float, 8>(row, c, n, f); }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = 0.f;
+    }
+    __device__ __forceinline__ float amax() const {
+        float m = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(f[j]));
+        return m;
+    }
+    __device__ __forceinline__ float value(int j) const { return f[j]; }
+    __device__ __forceinline__ void codes(float scale, uint32_t (&q)[2]) const {
+        q[0] = codes4(f[0], f[1], f[2], f[3], scale);
+        q[1] = codes4(f[4], f[5], f[6], f[7], scale);
+    }
+    static __device__ __forceinline__ uint32_t down(const Eight (&v)[8], int r, int j, float scale) {
+        return codes4(v[r].f[j], v[r + 1].f[j], v[r + 2].f[j], v[r + 3].f[j], scale);
+    }
+    static __device__ __forceinline__ void columns(const Eight (&v)[8], float (&m)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            m[j] = 0.f;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) m[j] = fmaxf(m[j], finite_abs(v[r].f[j]));
+        }
+    }
+};
+
 // Rows alone: 16 lanes hold a block of 128 columns.  Bound by memory; 16 blocks a
 // workgroup, so that a batch of few rows is spread over the chip.
 template <typename T> __global__ __launch_bounds__(256) void k_quantize_rows(QuantArgs a) {
-    const int64_t nb = (a.cols + BLK - 1) / BLK, total = a.rows * nb;
+    const int64_t nb = (a.cols + BLK - 1) / BLK, total = a.rows * nb, cend = (a.cols + 15) / 16 * 16;
     const int l = threadIdx.x & 15;
     for (int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); i < total; i += (int64_t)gridDim.x * 16) {
         const int64_t row = i / nb, kb = i % nb, c = kb * BLK + 8 * l;
-        float v[8], amax = 0.f;
-        ld_row<T, 8>((const T *)a.x + row * a.ld, c, a.cols, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(v[j]));
-        const int b = scale_byte(row16(amax, Max{}));
-        st_codes<8>(a.codes + row * a.codes_ld, c, a.codes_ld < nb * BLK ? a.codes_ld : nb * BLK, v, inv_scale(b));
+        Eight<T> v;
+        v.load((const T *)a.x + row * a.ld, c, a.cols);
+        const int b = scale_byte(row16(v.amax(), Max{}));
+        uint32_t q[2];
+        v.codes(scale_of(b), q);
+        st_codes<8>(a.codes + row * a.codes_ld, c, cend, q);
         if (l == 0) a.scale[row * a.scale_ld + kb] = (uint8_t)b;
     }
 }
@@ -53,62 +140,64 @@ template <typename T> __global__ __launch_bounds__(256) void k_quantize_rows(Qua
 // Thread (i, l) = (tid / 16, tid % 16) holds 8 rows x 8 columns: the amax of a row is
 // one over 16 neighbouring lanes, that of a column one over the 8 rows in registers,
 // then over the 16 threads above each other through LDS.  Transposed codes leave through
-// LDS in rows of 128 bytes.
+// LDS in rows of 128 bytes: word w (4 rows) of a column stands at w ^ swizzle(column), so
+// that neither the 16 columns 8 apart of a write nor a read's pieces of 8 columns meet in a bank.
 template <typename T, bool BLOCK>
 __global__ __launch_bounds__(256) void k_quantize_tile(QuantArgs a) {
-    __shared__ float red[16][BLK];
-    __shared__ uint32_t tr[BLK * 33];  // [column][32 words of 4 rows], pitch 33
+    __shared__ float red[16][BLK + 4];
+    __shared__ __align__(16) uint32_t tr[BLK * 32];
     const int l = threadIdx.x & 15, i = threadIdx.x >> 4;
     const int64_t r0 = (int64_t)blockIdx.y * BLK, c0 = (int64_t)blockIdx.x * BLK;
-    const int64_t c = c0 + 8 * l;
-    float v[8][8];
+    const int64_t c = c0 + 8 * l, cend = (a.cols + 15) / 16 * 16;
+    Eight<T> v[8];
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
         const int64_t row = r0 + 8 * i + r;
-        if (row < a.rows) {
-            ld_row<T, 8>((const T *)a.x + row * a.ld, c, a.cols, v[r]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[r][j] = 0.f;
-        }
+        if (row < a.rows) v[r].load((const T *)a.x + row * a.ld, c, a.cols);
+        else v[r].zero();
     }
     int bt[8];  // scale bytes of the transposed blocks of this thread's 8 columns
     int ball = 0;
     if (BLOCK || a.codes_t) {
+        float m[8];
+        Eight<T>::columns(v, m);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float m = 0.f;
-#pragma unroll
-            for (int r = 0; r < 8; ++r) m = fmaxf(m, finite_abs(v[r][j]));
-            red[i][8 * l + j] = m;
-        }
+        for (int j = 0; j < 8; ++j) red[i][8 * l + j] = m[j];
         __syncthreads();
-        float all = 0.f;
+        if constexpr (BLOCK) {
+            float all = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float m = 0.f;
+            for (int k = 0; k < 8; ++k) all = fmaxf(all, red[i][8 * l + k]);
+            all = row16(all, Max{});
+            if (l == 0) red[i][BLK] = all;
+            __syncthreads();
 #pragma unroll
-            for (int k = 0; k < 16; ++k) m = fmaxf(m, red[k][8 * l + j]);
-            bt[j] = scale_byte(m);
-            all = fmaxf(all, m);
+            for (int k = 0; k < 16; ++k) all = fmaxf(all, red[k][BLK]);
+            ball = scale_byte(all);
+        } else {
+            if (threadIdx.x < BLK) {
+                float x = 0.f;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) x = fmaxf(x, red[k][threadIdx.x]);
+                const int b = scale_byte(x);
+                red[0][threadIdx.x] = __builtin_bit_cast(float, b);
+                if (c0 + threadIdx.x < a.cols) a.scale_t[(c0 + threadIdx.x) * a.scale_t_ld + blockIdx.y] = (uint8_t)b;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) bt[j] = __builtin_bit_cast(int, red[0][8 * l + j]);
         }
-        if constexpr (BLOCK) ball = scale_byte(row16(all, Max{}));
-        __syncthreads();
     }
-    const int64_t cend = a.codes_ld < a.cols + (-a.cols & 15) ? a.codes_ld : a.cols + (-a.cols & 15);
     if (a.codes) {
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
             const int64_t row = r0 + 8 * i + r;
             int b = ball;
-            if constexpr (!BLOCK) {
-                float m = 0.f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(v[r][j]));
-                b = scale_byte(row16(m, Max{}));
-            }
+            if constexpr (!BLOCK) b = scale_byte(row16(v[r].amax(), Max{}));
             if (row < a.rows) {
-                st_codes<8>(a.codes + row * a.codes_ld, c, cend, v[r], inv_scale(b));
+                uint32_t q[2];
+                v[r].codes(scale_of(b), q);
+                st_codes<8>(a.codes + row * a.codes_ld, c, cend, q);
                 if (!BLOCK && l == 0) a.scale[row * a.scale_ld + blockIdx.x] = (uint8_t)b;
             }
         }
@@ -117,22 +206,25 @@ __global__ __launch_bounds__(256) void k_quantize_tile(QuantArgs a) {
     if (a.codes_t) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float inv = inv_scale(BLOCK ? ball : bt[j]);
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                tr[(8 * l + j) * 33 + 2 * i + h] = codes4(v[4 * h][j] * inv, v[4 * h + 1][j] * inv,
-                                                          v[4 * h + 2][j] * inv, v[4 * h + 3][j] * inv);
-            if (!BLOCK && i == 0 && c + j < a.cols) a.scale_t[(c + j) * a.scale_t_ld + blockIdx.y] = (uint8_t)bt[j];
+            const float scale = scale_of(BLOCK ? ball : bt[j]);
+            const int col = 8 * l + j;
+            uint2 q;
+            q.x = Eight<T>::down(v, 0, j, scale);
+            q.y = Eight<T>::down(v, 4, j, scale);
+            // 8-byte piece i of 16, swizzled within the row of 128 bytes
+            *(uint2 *)&tr[col * 32 + 2 * (i ^ (l & 15))] = q;
         }
         if (BLOCK && threadIdx.x == 0) a.scale_t[blockIdx.x * a.scale_t_ld + blockIdx.y] = (uint8_t)ball;
         __syncthreads();
         // codes_t_ld is a multiple of 16: pieces of 16 rows, zeros behind the last row
-        for (int p = threadIdx.x; p < BLK * 8; p += 256) {
-            const int col = p >> 3, piece = p & 7;
-            if (c0 + col < a.cols && r0 + 16 * piece < a.codes_t_ld) {
-                uint32_t q[4];
+        const int64_t rend = (a.rows + 15) / 16 * 16;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) q[k] = tr[col * 33 + 4 * piece + k];
+        for (int p = threadIdx.x; p < BLK * 8; p += 256) {
+            const int col = p >> 3, piece = p & 7, x = (col >> 3) & 15;
+            if (c0 + col < a.cols && r0 + 16 * piece < rend) {
+                uint2 q[2];
+                q[0] = *(const uint2 *)&tr[col * 32 + 2 * ((2 * piece) ^ x)];
+                q[1] = *(const uint2 *)&tr[col * 32 + 2 * ((2 * piece + 1) ^ x)];
                 __builtin_memcpy(a.codes_t + (c0 + col) * a.codes_t_ld + r0 + 16 * piece, q, 16);
             }
         }
@@ -143,7 +235,7 @@ __global__ __launch_bounds__(256) void k_quantize_tile(QuantArgs a) {
         for (int j = 0; j < 8; ++j) {
             float s = 0.f;
 #pragma unroll
-            for (int r = 0; r < 8; ++r) s += v[r][j];
+            for (int r = 0; r < 8; ++r) s += v[r].value(j);
             red[i][8 * l + j] = s;
         }
         __syncthreads();
@@ -156,21 +248,28 @@ __global__ __launch_bounds__(256) void k_quantize_tile(QuantArgs a) {
     }
 }
 
-// Codes [rows][cols] of any pitch and alignment to a pitch that is a multiple of 16, zeros behind
-// the last column.
-__global__ __launch_bounds__(256) void k_repack(const uint8_t *__restrict__ x, int64_t rows, int64_t cols, int64_t ld,
-                                                uint8_t *__restrict__ y, int64_t y_ld) {
-    const int64_t np = y_ld / 16, total = rows * np;
-    for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < total; p += (int64_t)gridDim.x * 256) {
-        const int64_t row = p / np, c = p % np * 16;
+// Codes of any pitch and alignment to a pitch y_ld that is a multiple of 16, zeros behind the last
+// column: up to two matrices in a launch.
+struct RepackArgs {
+    const uint8_t *x[2];
+    uint8_t *y[2];
+    int64_t rows[2], ld[2];
+    int64_t cols, y_ld;
+};
+__global__ __launch_bounds__(256) void k_repack(RepackArgs a) {
+    const int64_t np = a.y_ld / 16, first = a.rows[0] * np, total = first + a.rows[1] * np;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int which = i >= first;
+        const int64_t p = which ? i - first : i, row = p / np, c = p % np * 16;
+        const uint8_t *x = a.x[which] + row * a.ld[which] + c;
         uint8_t q[16];
-        if (c + 16 <= cols) {
-            __builtin_memcpy(q, x + row * ld + c, 16);
+        if (c + 16 <= a.cols) {
+            __builtin_memcpy(q, x, 16);
         } else {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) q[j] = c + j < cols ? x[row * ld + c + j] : 0;
+            for (int j = 0; j < 16; ++j) q[j] = c + j < a.cols ? x[j] : 0;
         }
-        __builtin_memcpy(y + row * y_ld + c, q, 16);
+        __builtin_memcpy(a.y[which] + row * a.y_ld + c, q, 16);
     }
 }
 
@@ -216,7 +315,6 @@ __device__ __forceinline__ void load_lds(const uint8_t *base, int size, int to, 
 // c += 2^(sa + sb) a b^T for lanes' fragments fb (rows of b: the tile's rows) and fa (rows of
 // a: its columns): 128 codes of a 16x16 tile, or 64 of a 32x32 one.  S: the scale's byte.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 struct Wide { bf16x8 v[4]; };  // 32 codes as bf16, their scale applied
 __device__ __forceinline__ Wide widen(const i32x8 &f, uint32_t s) {
@@ -627,21 +725,23 @@ __global__ __launch_bounds__(512) void k_block_matmul_few(SkinnyArgs s) {
                 uint32_t sa;
                 if constexpr (QUANT) {
                     const TX *row = (const TX *)s.x + mc * s.ldx;
-                    float v[4][8], amax = 0.f;
+                    Eight<TX> v[4];
+                    float amax = 0.f;
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
-                        ld_row<TX, 8>(row, k + 8 * p, a.K, v[p]);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(v[p][j]));
+                        v[p].load(row, k + 8 * p, a.K);
+                        amax = fmaxf(amax, v[p].amax());
                     }
                     amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
                     amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
                     sa = (uint32_t)scale_byte(amax);
-                    const float inv = inv_scale((int)sa);
+                    const float scale = scale_of((int)sa);
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
-                        fa[2 * p] = (int)codes4(v[p][0] * inv, v[p][1] * inv, v[p][2] * inv, v[p][3] * inv);
-                        fa[2 * p + 1] = (int)codes4(v[p][4] * inv, v[p][5] * inv, v[p][6] * inv, v[p][7] * inv);
+                        uint32_t q[2];
+                        v[p].codes(scale, q);
+                        fa[2 * p] = (int)q[0];
+                        fa[2 * p + 1] = (int)q[1];
                     }
                 } else {
                     fa = codes32(a.a + mc * a.lda, k);

@@ -90,22 +90,28 @@ __device__ __forceinline__ int scale_byte(float amax) {
     const int b = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u);
     return u == 0 ? 127 : b < 0 ? 0 : b;
 }
-// 2^-s of a scale byte (at most 247), and 2^s
-__device__ __forceinline__ float inv_scale(int b) { return __builtin_bit_cast(float, (uint32_t)(254 - b) << 23); }
+// 2^s of a scale byte
 __device__ __forceinline__ float scale_of(int b) { return __builtin_bit_cast(float, b ? (uint32_t)b << 23 : 1u << 22); }
 
-// four codes, round to nearest even (the instruction returns NaN for what is not finite)
-__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
-    int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+// four codes of values divided by scale, a power of two: round to nearest even, NaN for what is
+// not finite
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float scale) {
+    i16x2 r = {0, 0};
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a, b, scale, false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, scale, true);
+    return __builtin_bit_cast(uint32_t, r);
 }
-// codes c .. c+V-1 of a row whose V divides 128: all of them up to the row's end
-template <int V>
-__device__ __forceinline__ void st_codes(uint8_t *row, int64_t c, int64_t n, const float (&y)[V], float inv) {
-    uint32_t q[V / 4];
-#pragma unroll
-    for (int j = 0; j < V / 4; ++j)
-        q[j] = codes4(y[4 * j] * inv, y[4 * j + 1] * inv, y[4 * j + 2] * inv, y[4 * j + 3] * inv);
+// of two pairs of bf16
+__device__ __forceinline__ uint32_t codes4(uint32_t ab, uint32_t cd, float scale) {
+    i16x2 r = {0, 0};
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, ab), scale, false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2, cd), scale, true);
+    return __builtin_bit_cast(uint32_t, r);
+}
+// V codes from column c of a row on, those before column n
+template <int V> __device__ __forceinline__ void st_codes(uint8_t *row, int64_t c, int64_t n, const uint32_t (&q)[V / 4]) {
     if (c + V <= n) {
         __builtin_memcpy(row + c, q, V);
     } else {
@@ -113,6 +119,24 @@ __device__ __forceinline__ void st_codes(uint8_t *row, int64_t c, int64_t n, con
         for (int j = 0; j < V; ++j)
             if (c + j < n) row[c + j] = (uint8_t)(q[j / 4] >> (8 * (j & 3)));
     }
+}
+template <int V>
+__device__ __forceinline__ void st_codes(uint8_t *row, int64_t c, int64_t n, const float (&y)[V], float scale) {
+    uint32_t q[V / 4];
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) q[j] = codes4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3], scale);
+    st_codes<V>(row, c, n, q);
+}
+
+// Pairs of bf16 in words: |x| of finite elements (0 for the others) as 16-bit numbers, whose
+// order is theirs.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2 finite_abs2(uint32_t w) {
+    const i16x2 x = __builtin_bit_cast(i16x2, w & 0x7fff7fffu);
+    return __builtin_bit_cast(u16x2, x & ((x - (short)0x7f80) >> 15));
+}
+__device__ __forceinline__ float larger(u16x2 m) {
+    return __builtin_bit_cast(float, (uint32_t)(m[0] > m[1] ? m[0] : m[1]) << 16);
 }
 
 }  // namespace race

@@ -176,8 +176,9 @@ int mat_plan(const race_blocks *a, const race_blocks *b, int out_dtype, MatPlan 
     p.few = p.M <= kFewRows;
     if (p.few) {
         p.tn = (int)ceil_div(p.N, 16);
-        // workgroups of 8 waves: split the contraction until two a CU, each wave keeping two blocks
-        int64_t want = ceil_div(2 * kCUs, p.tn), most = ceil_div(p.ksteps, 16);
+        // Workgroups of 8 waves, one to 16 rows of b.  The sum of a split costs a launch, 4 us: it pays
+        // where few workgroups would walk many blocks each.
+        const int64_t want = ceil_div(kCUs, p.tn), most = ceil_div(p.ksteps, 8 * 8);
         p.splits = (int)(want < most ? want : most);
     } else {
         p.K = round_up(p.K, 16);
@@ -453,20 +454,28 @@ int race_block_matmul(const race_blocks *a, const race_blocks *b, const float *b
         else launch_few<bf16, false, float>(p, sk, s);
         return launched("race_block_matmul");
     }
-    auto repack = [&](const race_blocks *x, uint8_t *to) {
-        const int64_t n = ceil_div(x->rows * (p.K / 16), 256);
-        k_repack<<<(unsigned)(n < 65536 ? n : 65536), 256, 0, s>>>((const uint8_t *)x->codes, x->rows, x->cols, x->ld, to,
-                                                                    p.K);
-    };
-    if (p.pack_a) {
-        m.a = (const uint8_t *)ws;
-        m.lda = p.K;
-        repack(a, (uint8_t *)ws);
-    }
-    if (p.pack_b) {
-        m.b = (const uint8_t *)ws + p.pack_a;
-        m.ldb = p.K;
-        repack(b, (uint8_t *)ws + p.pack_a);
+    if (p.pack_a || p.pack_b) {
+        RepackArgs r{};
+        r.cols = a->cols;
+        r.y_ld = p.K;
+        auto add = [&](int i, const race_blocks *x, void *to) {
+            r.x[i] = (const uint8_t *)x->codes;
+            r.y[i] = (uint8_t *)to;
+            r.rows[i] = x->rows;
+            r.ld[i] = x->ld;
+        };
+        if (p.pack_a) {
+            add(0, a, ws);
+            m.a = r.y[0];
+            m.lda = p.K;
+        }
+        if (p.pack_b) {
+            add(1, b, (char *)ws + p.pack_a);
+            m.b = r.y[1];
+            m.ldb = p.K;
+        }
+        const int64_t n = ceil_div((r.rows[0] + r.rows[1]) * (p.K / 16), 256);
+        k_repack<<<(unsigned)(n < 65536 ? n : 65536), 256, 0, s>>>(r);
     }
     if (out_dtype == RACE_DTYPE_BF16) launch_tiles<bf16>(p, m, s);
     else launch_tiles<float>(p, m, s);

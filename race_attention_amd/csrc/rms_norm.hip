@@ -96,7 +96,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_rms_norm(NormArgs a) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) amax = fmaxf(amax, finite_abs(v[j]));
                 const int b = scale_byte(lanes<BLK / V>(amax, Max{}));
-                st_codes<V>((uint8_t *)a.y + row * a.ys, c, a.D, v, inv_scale(b));
+                st_codes<V>((uint8_t *)a.y + row * a.ys, c, a.D, v, scale_of(b));
                 if (c % BLK == 0 && c < a.D) a.scale[row * a.ss + c / BLK] = (uint8_t)b;
             } else {
                 st_row<TX, V>((TX *)a.y + row * a.ys, c, a.D, v);
