@@ -309,8 +309,7 @@ int race_quantize(const void *x, int32_t dtype, int64_t rows, int64_t cols, int6
  * in fp32; a bf16 one by the 8-bit matrix instructions, whose sums of 128 products are about
  * 2e-5 of their norm off (a bf16 step: 4e-3).  Codes
  * of any pitch and alignment; those that are whole 16-byte pieces are read in place, others are
- * copied to the workspace first (a of more than race_block_linear_rows() rows).  Workspace 0: ws
- * may be NULL. */
+ * copied to the workspace first (a of more than 32 rows).  Workspace 0: ws may be NULL. */
 size_t race_block_matmul_workspace_bytes(const race_blocks *a, const race_blocks *b, int32_t out_dtype);
 int race_block_matmul(const race_blocks *a, const race_blocks *b, const float *bias, void *out,
                       int32_t out_dtype, int64_t out_ld, void *ws, size_t ws_bytes, void *stream);

@@ -34,36 +34,22 @@ struct QuantArgs {
 // Elements of 8 columns as the quantisers hold them: bf16 as it is, in pairs, for which
 // comparing and converting take an instruction a pair, or fp32.
 template <typename T> struct Eight;
-template <> struct Eight<bf16> {
-    uint32_t w[4];
-    __device__ __forceinline__ void load(const bf16 *row, int64_t c, int64_t n) {
-        if (c + 8 <= n) {
-            __builtin_memcpy(w, row + c, 16);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                w[j] = 0;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    uint16_t x = 0;
-                    if (c + 2 * j + k < n) __builtin_memcpy(&x, row + c + 2 * j + k, 2);
-                    w[j] |= (uint32_t)x << (16 * k);
-                }
-            }
-        }
-    }
+template <> struct Eight<bf16> : Raw<bf16, 8> {
     __device__ __forceinline__ void zero() {
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = 0;
     }
+    // (what is not finite is larger than all that is: looked for only where it shows)
     __device__ __forceinline__ float amax() const {
-        u16x2 m = finite_abs2(w[0]);
+        u16x2 m = abs2(w[0]);
 #pragma unroll
-        for (int j = 1; j < 4; ++j) m = __builtin_elementwise_max(m, finite_abs2(w[j]));
+        for (int j = 1; j < 4; ++j) m = __builtin_elementwise_max(m, abs2(w[j]));
+        if (__builtin_expect(m[0] >= 0x7f80 || m[1] >= 0x7f80, 0)) {
+            m = finite_abs2(w[0]);
+#pragma unroll
+            for (int j = 1; j < 4; ++j) m = __builtin_elementwise_max(m, finite_abs2(w[j]));
+        }
         return larger(m);
-    }
-    __device__ __forceinline__ float value(int j) const {
-        return __builtin_bit_cast(float, j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
     }
     __device__ __forceinline__ void codes(float scale, uint32_t (&q)[2]) const {
         q[0] = codes4(w[0], w[1], scale);
@@ -87,9 +73,7 @@ template <> struct Eight<bf16> {
         }
     }
 };
-template <> struct Eight<float> {
-    float f[8];
-    __device__ __forceinline__ void load(const float *row, int64_t c, int64_t n) { ld_row<float, 8>(row, c, n, f); }
+template <> struct Eight<float> : Raw<float, 8> {
     __device__ __forceinline__ void zero() {
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = 0.f;
@@ -100,7 +84,6 @@ template <> struct Eight<float> {
         for (int j = 0; j < 8; ++j) m = fmaxf(m, finite_abs(f[j]));
         return m;
     }
-    __device__ __forceinline__ float value(int j) const { return f[j]; }
     __device__ __forceinline__ void codes(float scale, uint32_t (&q)[2]) const {
         q[0] = codes4(f[0], f[1], f[2], f[3], scale);
         q[1] = codes4(f[4], f[5], f[6], f[7], scale);
@@ -235,7 +218,7 @@ __global__ __launch_bounds__(256) void k_quantize_tile(QuantArgs a) {
         for (int j = 0; j < 8; ++j) {
             float s = 0.f;
 #pragma unroll
-            for (int r = 0; r < 8; ++r) s += v[r].value(j);
+            for (int r = 0; r < 8; ++r) s += v[r][j];
             red[i][8 * l + j] = s;
         }
         __syncthreads();
@@ -659,13 +642,13 @@ template <typename TO> __global__ __launch_bounds__(256) void k_split_sum(MatArg
 }
 
 // ------------------------------------------------------------ few rows
-// Up to 64 rows of a (single tokens): bound by the bytes of b, which no two workgroups
+// Up to 32 rows of a (single tokens): bound by the bytes of b, which no two workgroups
 // share.  A workgroup owns 16 rows of b; its 8 waves split the contraction (and, where
 // that leaves the chip empty, so does the grid), read b from memory straight into the
 // matrix cores' operands (a lane 32 consecutive bytes of a row, 128 bytes a row and
 // instruction), and add their tiles through LDS in the waves' order.
-// QUANT: a is bf16 or fp32 and is quantised on the way (its blocks' 128 values are in 4
-// lanes), which saves the quantiser's launch; every workgroup repeats it for its share.
+// QUANT (up to 16 rows): a is bf16 or fp32 and is quantised on the way (its blocks' 128 values
+// are in 4 lanes), which saves the quantiser's launch; every workgroup repeats it for its share.
 struct SkinnyArgs {
     MatArgs m;
     const void *x;
@@ -688,66 +671,75 @@ __global__ __launch_bounds__(512) void k_block_matmul_few(SkinnyArgs s) {
     // 32 bytes k .. k+31 of a row of codes, zeros from K on
     auto codes32 = [&](const uint8_t *row, int64_t k) {
         i32x8 f;
-        if (k + 32 <= a.K) {
+        if (no_lane(k + 32 > a.K)) {
             __builtin_memcpy(&f, row + k, 32);
         } else {
+            const int left = left_in_row<32>(k, a.K);
+            const uint8_t *p = row + (left ? k : 0);
+            uint8_t t[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) t[j] = p[j < left ? j : 0];
 #pragma unroll
             for (int w = 0; w < 8; ++w) {
                 uint32_t v = 0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (k + 4 * w + j < a.K) v |= (uint32_t)row[k + 4 * w + j] << (8 * j);
+                for (int j = 0; j < 4; ++j) v |= (4 * w + j < left ? (uint32_t)t[4 * w + j] : 0u) << (8 * j);
                 f[w] = (int)v;
             }
         }
         return f;
     };
-    constexpr int U = MT <= 2 ? 4 : 2;  // blocks in flight
+    constexpr int U = 4;  // blocks of b in flight, and of 16 rows of a
     for (int kb = kb0 + wave; kb < kb1; kb += WAVES * U) {
         i32x8 fb[U];
         uint32_t sb[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int k1 = kb + u * WAVES, kc = k1 < kb1 ? k1 : kb;
+            const int k1 = kb + u * WAVES, kc = k1 < kb1 ? k1 : kb0;
             fb[u] = codes32(brow, (int64_t)kc * BLK + 32 * q);
             sb[u] = sbrow[kc];
+            // behind the wave's last block: zeros times the row's first one, whose NaN are the row's anyway
+            // (no branch below, so that all loads are on their way at once)
+            if (k1 >= kb1) fb[u] = i32x8{0, 0, 0, 0, 0, 0, 0, 0};
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int k1 = kb + u * WAVES;
-            if (k1 >= kb1) break;
-            const int64_t k = (int64_t)k1 * BLK + 32 * q;
-            const auto wb = Operand<TO>::of(fb[u], sb[u]);
+        for (int i = 0; i < MT; ++i) {
+            const int64_t m = 16 * i + i16, mc = m < a.M ? m : a.M - 1;
+            std::conditional_t<QUANT, Eight<TX>, int> x[U][4];
+            i32x8 fa[U];
+            uint32_t sa[U];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int64_t m = 16 * i + i16, mc = m < a.M ? m : a.M - 1;
-                i32x8 fa;
-                uint32_t sa;
+            for (int u = 0; u < U; ++u) {
+                const int k1 = kb + u * WAVES, kc = k1 < kb1 ? k1 : kb0;
+                const int64_t k = (int64_t)kc * BLK + 32 * q;
                 if constexpr (QUANT) {
                     const TX *row = (const TX *)s.x + mc * s.ldx;
-                    Eight<TX> v[4];
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) x[u][p].load(row, k + 8 * p, a.K);
+                } else {
+                    fa[u] = codes32(a.a + mc * a.lda, k);
+                    sa[u] = a.sa[(mc >> a.sha) * a.lsa + kc];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if constexpr (QUANT) {
                     float amax = 0.f;
 #pragma unroll
-                    for (int p = 0; p < 4; ++p) {
-                        v[p].load(row, k + 8 * p, a.K);
-                        amax = fmaxf(amax, v[p].amax());
-                    }
+                    for (int p = 0; p < 4; ++p) amax = fmaxf(amax, x[u][p].amax());
                     amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
                     amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
-                    sa = (uint32_t)scale_byte(amax);
-                    const float scale = scale_of((int)sa);
+                    sa[u] = (uint32_t)scale_byte(amax);
+                    const float scale = scale_of((int)sa[u]);
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
-                        uint32_t q[2];
-                        v[p].codes(scale, q);
-                        fa[2 * p] = (int)q[0];
-                        fa[2 * p + 1] = (int)q[1];
+                        uint32_t c[2];
+                        x[u][p].codes(scale, c);
+                        fa[u][2 * p] = (int)c[0];
+                        fa[u][2 * p + 1] = (int)c[1];
                     }
-                } else {
-                    fa = codes32(a.a + mc * a.lda, k);
-                    sa = a.sa[(mc >> a.sha) * a.lsa + k1];
                 }
-                acc[i] = block_product(wb, Operand<TO>::of(fa, sa), acc[i]);
+                acc[i] = block_product(Operand<TO>::of(fb[u], sb[u]), Operand<TO>::of(fa[u], sa[u]), acc[i]);
             }
         }
     }

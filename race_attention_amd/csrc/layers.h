@@ -37,14 +37,64 @@ template <typename T, int V> __device__ __forceinline__ void st_vec(T *p, const 
     for (int j = 0; j < V; ++j) t[j] = (T)r[j];
     __builtin_memcpy(p, t, sizeof t);
 }
-// elements c .. c+V-1 of a row of n: zeros behind its end
-template <typename T, int V> __device__ __forceinline__ void ld_row(const T *row, int64_t c, int64_t n, float (&r)[V]) {
-    if (c + V <= n) {
-        ld_vec<T, V>(row + c, r);
+// whether a condition holds in none of the wave's active lanes: a branch on it is the wave's, so its
+// other side costs nothing
+__device__ __forceinline__ bool no_lane(bool x) { return __builtin_amdgcn_ballot_w64(x) == 0; }
+// elements of the row from c on, 0 to V, as a number that the compiler does not form before the
+// branch that uses it
+template <int V> __device__ __forceinline__ int left_in_row(int64_t c, int64_t n) {
+    int left = n - c < V ? (int)(n - c) : V;
+    left = left < 0 ? 0 : left;
+    asm volatile("" : "+v"(left));
+    return left;
+}
+// elements c .. c+V-1 of a row of n >= 1: zeros behind its end.  (A wave that reaches it loads elements
+// one by one, the first again in place of what lies behind it: loads under a condition each would wait
+// for each other.)
+template <typename T, int V> __device__ __forceinline__ void ld_raw(const T *row, int64_t c, int64_t n, T (&t)[V]) {
+    if (no_lane(c + V > n)) {
+        __builtin_memcpy(t, row + c, sizeof t);
     } else {
+        const int left = left_in_row<V>(c, n);
+        const T *p = row + (left ? c : 0);
 #pragma unroll
-        for (int j = 0; j < V; ++j) r[j] = c + j < n ? (float)row[c + j] : 0.f;
+        for (int j = 0; j < V; ++j) t[j] = p[j < left ? j : 0];
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[j] = j < left ? t[j] : (T)0.f;
     }
+}
+// V elements as they were loaded, in whole registers (bf16 in pairs)
+template <typename T, int V> struct Raw;
+template <int V> struct Raw<float, V> {
+    float f[V];
+    __device__ __forceinline__ void load(const float *row, int64_t c, int64_t n) { ld_raw<float, V>(row, c, n, f); }
+    __device__ __forceinline__ float operator[](int j) const { return f[j]; }
+};
+template <int V> struct Raw<bf16, V> {
+    uint32_t w[V / 2];
+    __device__ __forceinline__ void load(const bf16 *row, int64_t c, int64_t n) {
+        if (no_lane(c + V > n)) {
+            __builtin_memcpy(w, row + c, sizeof w);
+        } else {
+            const int left = left_in_row<V>(c, n);
+            const bf16 *p = row + (left ? c : 0);
+            uint16_t t[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) __builtin_memcpy(&t[j], p + (j < left ? j : 0), 2);
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j)
+                w[j] = (2 * j < left ? t[2 * j] : 0u) | (uint32_t)(2 * j + 1 < left ? t[2 * j + 1] : 0u) << 16;
+        }
+    }
+    __device__ __forceinline__ float operator[](int j) const {
+        return __builtin_bit_cast(float, j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+    }
+};
+template <typename T, int V> __device__ __forceinline__ void ld_row(const T *row, int64_t c, int64_t n, float (&r)[V]) {
+    T t[V];
+    ld_raw<T, V>(row, c, n, t);
+#pragma unroll
+    for (int j = 0; j < V; ++j) r[j] = (float)t[j];
 }
 template <typename T, int V> __device__ __forceinline__ void st_row(T *row, int64_t c, int64_t n, const float (&r)[V]) {
     if (c + V <= n) {
@@ -131,6 +181,7 @@ __device__ __forceinline__ void st_codes(uint8_t *row, int64_t c, int64_t n, con
 // Pairs of bf16 in words: |x| of finite elements (0 for the others) as 16-bit numbers, whose
 // order is theirs.
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2 abs2(uint32_t w) { return __builtin_bit_cast(u16x2, w & 0x7fff7fffu); }
 __device__ __forceinline__ u16x2 finite_abs2(uint32_t w) {
     const i16x2 x = __builtin_bit_cast(i16x2, w & 0x7fff7fffu);
     return __builtin_bit_cast(u16x2, x & ((x - (short)0x7f80) >> 15));

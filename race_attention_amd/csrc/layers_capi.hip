@@ -53,11 +53,13 @@ unsigned norm_grid(int64_t rows, int rpb) {
     const int64_t n = ceil_div(rows, rpb);
     return (unsigned)(n < (1 << 20) ? n : 1 << 20);
 }
-// of the backward, each with a row of dw_part: 4 of 256 threads per CU keep enough loads in
-// flight; more only add to the parts that are summed afterwards
+// of the backward, each with a row of dw_part: as many as keep the memory busy, and no more, because
+// their parts are written and added.  us at 512, 768 and 1024: 65536 x 768 bf16 100, 101, 111; 8192 x
+// 4096 67, 77, 73; 4001 x 1001 fp32 17, 20, 23; 50240 x 384 fp32 104, 87, 82 (short rows: little of one is on
+// its way at a time).
 int64_t norm_bwd_grid(int64_t rows, int64_t D) {
-    const int64_t n = ceil_div(rows, D <= 1024 ? 4 : 1);
-    return n < 1024 ? n : 1024;
+    const int64_t n = ceil_div(rows, D <= 1024 ? 4 : 1), most = D <= 512 ? 1024 : 512;
+    return n < most ? n : most;
 }
 
 // f<V, NV, L>() for a row length: a wave up to 1024 columns, a workgroup up to 16384
@@ -152,12 +154,16 @@ int check_out_blocks(const char *name, const race_blocks *b) {
 struct MatPlan {
     int M, N;            // rows of a, of b
     int64_t K;           // contraction, as the kernels see it
-    int ksteps, few;     // blocks along K; few: the kernel for up to 64 rows
+    int ksteps, few;     // blocks along K; few: the kernel for few rows
     int bm, bn, tm, tn, splits, kper;
     size_t pack_a, pack_b, parts;  // workspace: repacked operands, parts of a split contraction
 };
 
-constexpr int kFewRows = 64;
+// Rows of a up to which k_block_matmul_few multiplies, and up to which it also quantises: every
+// workgroup repeats that, so from 17 rows on a launch of its own is faster (us, 4096 x 4096, 16 rows: 11.5
+// against 14.1; 32: 15.7 and 14.2).  From 33 rows on tiles of 128 are as fast or faster: 64 rows
+// 19 against 17 for 4096 x 4096, 26 against 55 for 8192 x 8192.
+constexpr int kFewRows = 32, kLinearRows = 16;
 constexpr int kCUs = 256;
 
 bool direct(const race_blocks *b) { return b->ld % 16 == 0 && b->cols % 16 == 0 && (uintptr_t)b->codes % 16 == 0; }
@@ -198,7 +204,8 @@ int mat_plan(const race_blocks *a, const race_blocks *b, int out_dtype, MatPlan 
         p.bm = 256;
         for (int s = 1; s == 1 || (s <= 64 && 2 * s <= p.ksteps && (s - 1) * small < 2 * kCUs); ++s) {
             const int64_t wgs = small * s;
-            const double step = wgs <= kCUs ? 0.65 : 1.0;
+            // (bf16 products of an fp32 output: 1.75 and 1.5)
+            const double step = out_dtype == RACE_DTYPE_F32 ? (wgs <= kCUs ? 1.5 : 1.75) : wgs <= kCUs ? 0.65 : 1.0;
             const double t = (double)ceil_div(wgs, 2 * kCUs) * (step * ceil_div(p.ksteps, s) + 4) +
                              (s > 1 ? 4 + 2e-6 * s * p.M * p.N : 0.0);
             if (t < best) {
@@ -237,9 +244,8 @@ template <typename TO> void launch_tiles(const MatPlan &p, const MatArgs &m, hip
 template <typename TX, bool QUANT, typename TO>
 void launch_few(const MatPlan &p, const SkinnyArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)p.tn, (unsigned)p.splits);
-    if (p.M <= 16) k_block_matmul_few<1, TX, QUANT, TO><<<grid, 512, 0, s>>>(a);
-    else if (p.M <= 32) k_block_matmul_few<2, TX, QUANT, TO><<<grid, 512, 0, s>>>(a);
-    else k_block_matmul_few<4, TX, QUANT, TO><<<grid, 512, 0, s>>>(a);
+    if (QUANT || p.M <= 16) k_block_matmul_few<1, TX, QUANT, TO><<<grid, 512, 0, s>>>(a);
+    else k_block_matmul_few<2, TX, false, TO><<<grid, 512, 0, s>>>(a);
     if (p.splits > 1) launch_sum<TO>(a.m, p.splits, s);
 }
 
@@ -482,11 +488,11 @@ int race_block_matmul(const race_blocks *a, const race_blocks *b, const float *b
     return launched("race_block_matmul");
 }
 
-int64_t race_block_linear_rows(void) { return kFewRows; }
+int64_t race_block_linear_rows(void) { return kLinearRows; }
 
 size_t race_block_linear_workspace_bytes(int64_t rows, const race_blocks *b, int32_t out_dtype) {
-    if (!b || rows < 1 || rows > kFewRows) {
-        fail(RACE_E_INVALID, "1 to %d rows (got %lld) and a matrix b", kFewRows, (ll)rows);
+    if (!b || rows < 1 || rows > kLinearRows) {
+        fail(RACE_E_INVALID, "1 to %d rows (got %lld) and a matrix b", kLinearRows, (ll)rows);
         return 0;
     }
     race_blocks a = *b;
@@ -498,8 +504,8 @@ int race_block_linear(const void *x, int32_t dtype, int64_t rows, int64_t x_ld, 
                       void *out, int32_t out_dtype, int64_t out_ld, void *ws, size_t ws_bytes, void *stream) {
     int rc;
     if (!dtype_ok(dtype)) return fail(RACE_E_INVALID, "dtype %d is not RACE_DTYPE_F32 or RACE_DTYPE_BF16", dtype);
-    if (rows < 1 || rows > kFewRows)
-        return fail(RACE_E_UNSUPPORTED, "rows=%lld: 1 to %d (quantise more rows first)", (ll)rows, kFewRows);
+    if (rows < 1 || rows > kLinearRows)
+        return fail(RACE_E_UNSUPPORTED, "rows=%lld: 1 to %d (quantise more rows first)", (ll)rows, kLinearRows);
     if ((rc = check_blocks("b", b))) return rc;
     if ((rc = check_rows("x", x, esize(dtype), rows, b->cols, x_ld, false))) return rc;
     race_blocks a = *b;  // sizes alone: x takes its codes' place
