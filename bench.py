@@ -41,7 +41,8 @@ AdamW; bf16 autocast over fp32 weights): the ViT encoder (6 layers, d=384,
 6 heads, MLP 1536, non-causal K=2 L=5 M=1, batch 64 x 785 tokens of 28x28
 images, 10 classes) and the GPT decoder (12 layers, d=768, 12 heads, MLP
 3072, vocab 50257, causal K=8 L=4 M=2, batch 8 x 8192 token ids).  Value is
-tokens/s of the step.
+tokens/s of the step.  --norm rms, --linear fp8 and --optimizer adamw32 | adamw8
+put this package's operators in the blocks and the step.
 
 --copy-calib MIB ends the run with one device-to-device copy of MIB MiB, the
 known-size kernel against which rocprofv3's FETCH_SIZE / WRITE_SIZE counters
@@ -83,6 +84,11 @@ def parse():
     ap.add_argument("--copy-calib", type=int, default=0, metavar="MIB",
                     help="finish with a device-to-device copy of MIB MiB (PMC calibration)")
     ap.add_argument("--workload", choices=("c4", "c5", "c3-step", "c5-step"), default="c4")
+    ap.add_argument("--norm", choices=("layer", "rms"), default="layer",
+                    help="model steps: the blocks' norms (rms: root mean square, adding the residual)")
+    ap.add_argument("--linear", choices=("torch", "fp8"), default="torch", help="model steps: the blocks' linear layers")
+    ap.add_argument("--optimizer", choices=("torch", "adamw32", "adamw8"), default="torch",
+                    help="model steps: torch's AdamW, or this package's with states in 32 or 8 bits")
     ap.add_argument("--mode", choices=("f1", "global", "probs"), default="f1",
                     help="f1: per-bucket normalisation (headline); global: one normaliser per token; "
                          "probs: the bucket probabilities of Q as an output, forward + backward")
@@ -259,10 +265,11 @@ def model_step_main(args):
     import torch
     dev = torch.device("cuda:0")
     torch.manual_seed(0)
+    ops = dict(norm=args.norm, linear=args.linear)
     if args.workload == "c3-step":
         from race_attention_amd.vit import VisionTransformer
         cfg = dict(img_size=28, patch_size=1, num_channels=1, embed_dim=384, num_heads=6, transformer_units=6,
-                   drop_rate=0.1, qkv_bias=False, K=2, L=5, M=1, num_classes=10)
+                   drop_rate=0.1, qkv_bias=False, K=2, L=5, M=1, num_classes=10, **ops)
         model = VisionTransformer(cfg).to(dev)
         B, T = 64, 28 * 28 + 1
         x = torch.randn(B, 1, 28, 28, device=dev)
@@ -272,14 +279,21 @@ def model_step_main(args):
     else:
         from race_attention_amd.lm import LMModel
         cfg = dict(vocab_size=50257, context_length=8192, emb_dim=768, n_heads=12, n_layers=12, drop_rate=0.1,
-                   qkv_bias=False, K=8, L=4, M=2)
+                   qkv_bias=False, K=8, L=4, M=2, **ops)
         model = LMModel(cfg).to(dev)
         B, T = 8, 8192
         x = torch.randint(0, 50257, (B, T), device=dev)
         y = torch.randint(0, 50257, (B, T), device=dev)
         loss_fn = lambda out: torch.nn.functional.cross_entropy(out.flatten(0, 1), y.flatten())  # noqa: E731
         wl = "C5 GPT training step (12 causal RACE blocks, d=768, 12 heads, K=8 L=4 M=2, vocab 50257), AdamW"
-    opt = torch.optim.AdamW(model.parameters(), lr=6e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1)
+    hyper = dict(lr=6e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1)
+    if args.optimizer == "torch":
+        opt = torch.optim.AdamW(model.parameters(), **hyper)
+    else:
+        from race_attention_amd.optim import AdamW
+        opt = AdamW(model.parameters(), bits=8 if args.optimizer == "adamw8" else 32, **hyper)
+    if (args.norm, args.linear, args.optimizer) != ("layer", "torch", "torch"):
+        wl += f", norm {args.norm}, linear {args.linear}, optimizer {args.optimizer}"
     print(f"bench: {wl}: {sum(p.numel() for p in model.parameters())} parameters", file=sys.stderr, flush=True)
 
     def step():

@@ -292,7 +292,8 @@ typedef struct race_blocks {
     int32_t block_rows;   /* 1 or 128 */
 } race_blocks;
 
-/* The norm's y in 8-bit blocks (block_rows = 1), with pitch and codes as race_quantize. */
+/* The norm's y in 8-bit blocks (block_rows = 1), pitch and alignment as race_quantize's; bytes
+ * behind a row's last code are not written. */
 int race_rms_norm_codes(const race_norm_desc *d, const void *x, const void *residual, const float *w,
                         const race_blocks *y, void *h, void *stream);
 

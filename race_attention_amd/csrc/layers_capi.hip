@@ -186,6 +186,8 @@ int mat_plan(const race_blocks *a, const race_blocks *b, int out_dtype, MatPlan 
         // where few workgroups would walk many blocks each.
         const int64_t want = ceil_div(kCUs, p.tn), most = ceil_div(p.ksteps, 8 * 8);
         p.splits = (int)(want < most ? want : most);
+        if ((int64_t)p.tn * 512 * (p.splits < 1 ? 1 : p.splits) >= (int64_t)1 << 32)
+            return fail(RACE_E_UNSUPPORTED, "%d rows of b exceed one launch's 2^32 work-items", p.N);
     } else {
         p.K = round_up(p.K, 16);
         if (!direct(a)) p.pack_a = align256((size_t)(a->rows * p.K));

@@ -25,8 +25,23 @@ struct Layers {
 #undef X
 } lib;
 
+// A status that is an error: in a forward call the Python path makes the call again and raises it
+// (NotTaken), the engine's thread raises it itself.
+struct Status : NotTaken {
+    const char *what;
+    int rc;
+    std::string text;
+};
 void check(const char *what, int rc) {
-    if (rc != RACE_OK) raise_race_error(what, rc, lib.race_last_error());
+    if (rc != RACE_OK) throw Status{{}, what, rc, lib.race_last_error()};
+}
+template <typename F> variable_list backward_of(F &&f) {
+    try {
+        at::NoGradGuard ng;
+        return f();
+    } catch (const Status &s) {
+        raise_race_error(s.what, s.rc, s.text.c_str());
+    }
 }
 
 constexpr int64_t BLOCK = 128;
@@ -110,9 +125,7 @@ struct Norm : torch::autograd::Function<Norm> {
         const auto saved = ctx->get_saved_variables();
         Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
         if (!dy.defined() && !dh.defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-        variable_list out;
-        {
-            at::NoGradGuard ng;
+        return once(backward_of([&]() -> variable_list {
             const Tensor x2 = saved[0].defined() ? rows2d(saved[0]) : Tensor(), r = saved[1], r2 = rows2d(r), &w = saved[2];
             const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
             const Tensor dy2 = rows2d(dy.defined() ? dy.to(type) : at::zeros(r.sizes(), r.options().dtype(type)));
@@ -137,11 +150,10 @@ struct Norm : torch::autograd::Function<Norm> {
                   lib.race_rms_norm_bwd(&d, x2.defined() ? ptr(x2) : nullptr, ptr(r2), fptr(w32), fptr(saved[3]), ptr(dy2),
                                         dh2.defined() ? ptr(dh2) : nullptr, ptr(dx), dr.is_same(dx) ? nullptr : ptr(dr),
                                         fptr(dw), ptr(ws), (size_t)ws.numel(), stream_of(r)));
-            out = {ctx->needs_input_grad(0) ? dx : Tensor(),
-                   ctx->needs_input_grad(1) ? dw.to(w.scalar_type()) : Tensor(),
-                   ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(2) ? dr : Tensor(), Tensor()};
-        }
-        return once(out);
+            return {ctx->needs_input_grad(0) ? dx : Tensor(),
+                    ctx->needs_input_grad(1) ? dw.to(w.scalar_type()) : Tensor(),
+                    ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(2) ? dr : Tensor(), Tensor()};
+        }));
     }
 };
 
@@ -283,9 +295,7 @@ struct Linear : torch::autograd::Function<Linear> {
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        variable_list out;
-        {
-            at::NoGradGuard ng;
+        return once(backward_of([&]() -> variable_list {
             auto is = [&](const char *k) { return ctx->saved_data[k].toInt(); };
             const std::vector<int64_t> shape = ctx->saved_data["shape"].toIntVector();
             const bool need_x = ctx->saved_data["need_x"].toBool(), need_w = ctx->saved_data["need_w"].toBool();
@@ -297,9 +307,8 @@ struct Linear : torch::autograd::Function<Linear> {
             if (need_w)
                 dw = product(q.t, Blocks{saved[0], saved[1], 1}, {dy2.size(1), shape.back()}, Tensor(),
                              (at::ScalarType)is("w"));
-            out = {dx, dw, bt >= 0 ? q.sums.to((at::ScalarType)bt) : Tensor(), Tensor()};
-        }
-        return once(out);
+            return {dx, dw, bt >= 0 ? q.sums.to((at::ScalarType)bt) : Tensor(), Tensor()};
+        }));
     }
 };
 
@@ -323,6 +332,19 @@ bool bias_arg(py::handle h, int64_t N, Tensor &bias) {
     return optional_arg(h, bias) && (!bias.defined() || (bias.dim() == 1 && bias.size(0) == N &&
                                                          at::isFloatingType(bias.scalar_type())));
 }
+// f()'s tensor without the interpreter's lock, or None where its call was not taken
+template <typename F> py::object taken(F &&f) {
+    try {
+        Tensor out;
+        {
+            py::gil_scoped_release nogil;
+            out = f();
+        }
+        return py::cast(out);
+    } catch (const NotTaken &) {
+        return py::none();
+    }
+}
 at::ScalarType type_of(bool fp32_out) { return fp32_out ? at::kFloat : at::kBFloat16; }
 
 py::object matmul(py::handle ac, py::handle as, int64_t ar, py::handle bc, py::handle bs, int64_t br, py::handle hbias,
@@ -332,19 +354,15 @@ py::object matmul(py::handle ac, py::handle as, int64_t ar, py::handle bc, py::h
     if (redirected() || !block_args(ac, as, ar, a, false) || !block_args(bc, bs, br, b, true) ||
         a.codes.size(-1) != b.codes.size(1) || !bias_arg(hbias, b.codes.size(0), bias))
         return py::none();
-    py::gil_scoped_release nogil;
-    Tensor out;
-    {
+    return taken([&]() -> Tensor {
         at::NoGradGuard ng;
         const auto shape = out_shape(a.codes, b.codes.size(0));
         a.codes = rows2d(a.codes);
         a.scale = rows2d(a.scale);
         b.codes = rows2d(b.codes);
         b.scale = rows2d(b.scale);
-        out = product(a, b, shape, bias.defined() ? f32(bias) : bias, type_of(fp32_out));
-    }
-    py::gil_scoped_acquire gil;
-    return py::cast(out);
+        return product(a, b, shape, bias.defined() ? f32(bias) : bias, type_of(fp32_out));
+    });
 }
 
 // weight: a tensor (hs None), or codes and scales of 128 x 128 or 1 x 128 blocks
@@ -364,11 +382,8 @@ py::object linear(py::handle hx, py::handle hw, py::handle hs, int64_t block_row
     const bool grad = frozen ? wants_grad({&x, &bias}) : wants_grad({&x, &w, &bias});
     if (grad && (frozen || R > ((int64_t)1 << 22) - 16)) return py::none();
     const at::ScalarType type = type_of(fp32_out);
-    py::gil_scoped_release nogil;
-    Tensor y;
-    if (grad) {
-        y = Linear::apply(x, w, given(bias), (int64_t)type);
-    } else {
+    return taken([&]() -> Tensor {
+        if (grad) return Linear::apply(x, w, given(bias), (int64_t)type);
         at::NoGradGuard ng;
         const Tensor x2 = rows2d(x), b32 = bias.defined() ? f32(bias) : Tensor();
         if (frozen) {
@@ -377,21 +392,18 @@ py::object linear(py::handle hx, py::handle hw, py::handle hs, int64_t block_row
         } else {
             b = quantize(rows2d(w), BLOCK, true, false, false).y;
         }
-        y = R <= lib.race_block_linear_rows() ? product_few(x2, b, out_shape(x, N), b32, type)
-                                              : product(quantize(x2, 1, true, false, false).y, b, out_shape(x, N), b32, type);
-    }
-    py::gil_scoped_acquire gil;
-    return py::cast(y);
+        if (R <= lib.race_block_linear_rows()) return product_few(x2, b, out_shape(x, N), b32, type);
+        return product(quantize(x2, 1, true, false, false).y, b, out_shape(x, N), b32, type);
+    });
 }
 
 // (codes, scale) or (codes, scale, h) of a norm in 8-bit blocks
 py::object rms_norm_codes(py::handle hx, py::handle hw, py::handle hr, double eps) {
     Tensor x, w, r;
     if (!norm_args(hx, hw, hr, x, w, r) || wants_grad({&x, &w, &r}) || x.dim() != 2) return py::none();
-    py::gil_scoped_release nogil;
     Blocks y;
     Tensor h;
-    {
+    const py::object done = taken([&]() -> Tensor {
         at::NoGradGuard ng;
         const Tensor x2 = rows2d(x), r2 = r.defined() ? rows2d(r) : r, w32 = f32(w);
         y = empty_blocks(x.size(0), x.size(1), 1, x);
@@ -401,8 +413,9 @@ py::object rms_norm_codes(py::handle hx, py::handle hw, py::handle hr, double ep
         check("race_rms_norm_codes",
               lib.race_rms_norm_codes(&d, ptr(x2), r2.defined() ? ptr(r2) : nullptr, fptr(w32), &b,
                                       h.defined() ? ptr(h) : nullptr, stream_of(x)));
-    }
-    py::gil_scoped_acquire gil;
+        return y.codes;
+    });
+    if (done.is_none()) return done;
     return h.defined() ? py::object(py::make_tuple(y.codes, y.scale, h)) : py::object(py::make_tuple(y.codes, y.scale));
 }
 
@@ -425,7 +438,8 @@ bool adamw(py::list ps, py::list gs, py::list ms, py::list vs, py::list mscales,
     std::vector<race_adamw_tensor> table(n);
     std::vector<Tensor> written;
     written.reserve(n * (eight ? 5 : 3));
-    std::vector<const void *> seen[3];
+    std::vector<const void *> seen;
+    seen.reserve(3 * n);
     Tensor p0, g0;
     for (size_t i = 0; i < n; ++i) {
         Tensor p, g, m, v, sm, sv;
@@ -462,18 +476,16 @@ bool adamw(py::list ps, py::list gs, py::list ms, py::list vs, py::list mscales,
             written.push_back(sv);
         }
         if (t.n) {
-            seen[0].push_back(t.p);
-            seen[1].push_back(t.m);
-            seen[2].push_back(t.v);
+            seen.push_back(t.p);
+            seen.push_back(t.m);
+            seen.push_back(t.v);
         }
         written.push_back(std::move(p));
         written.push_back(std::move(m));
         written.push_back(std::move(v));
     }
-    for (auto &s : seen) {
-        std::sort(s.begin(), s.end());
-        if (std::adjacent_find(s.begin(), s.end()) != s.end()) return false;  // twice in the lists: refused there
-    }
+    std::sort(seen.begin(), seen.end());
+    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) return false;  // twice in the lists: refused there
     d.lr = lr;
     d.beta_m = b1;
     d.beta_v = b2;

@@ -308,7 +308,8 @@ class Linear(nn.Linear):
 
     def freeze(self):
         """Quantise the weight as it is now; forward then uses the result, which has no gradient.
-        Loading a state_dict or moving the module quantises anew; unfreeze() goes back."""
+        Loading a state_dict, or another type or GPU, quantises anew; unfreeze() goes back, and so does
+        moving the module off the GPU."""
         self.frozen = quantize(self.weight.detach(), BLOCK)
         return self
 

@@ -16,6 +16,8 @@ from .race import RACEBlock, norm_of
 
 
 class LMModel(nn.Module):
+    fused = False  # root-mean-square norms that add the residual
+
     def __init__(self, cfg, attn_type="race", device="cpu"):
         super().__init__()
         if attn_type != "race":

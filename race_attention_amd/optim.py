@@ -79,7 +79,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
     captured graphs; it is then added to seed).  seed: of the 8-bit states' rounding; take another one
     each step.
 
-    A parameter or state that stands in the lists twice is refused."""
+    A parameter or state that stands in the lists twice is refused; ones that overlap otherwise must
+    not be given."""
     params, grads, ms, vs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
     if not len(params) == len(grads) == len(ms) == len(vs):
         raise ValueError("lists of different lengths")
@@ -111,10 +112,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas=(0.9, 0.
             t.m, t.m_scale, t.v, t.v_scale = (x.data_ptr() for s in (m, v) for x in (s.codes, s.scale))
         else:
             t.m, t.v = m.data_ptr(), v.data_ptr()
-    for name in ("p", "m", "v"):
-        at = [getattr(t, name) for t in table if t.n]
-        if len(set(at)) < len(at):
-            raise ValueError("a tensor stands in the lists twice")
+    at = [x for t in table if t.n for x in (t.p, t.m, t.v)]
+    if len(set(at)) < len(at):
+        raise ValueError("a tensor stands in the lists twice")
     d.p_dtype, d.g_dtype = DTYPES[p0.dtype], DTYPES[g0.dtype]
     with on_device(p0):
         rc = _lib.load().race_adamw(ctypes.byref(d), table, len(params), stream(p0))

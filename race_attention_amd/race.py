@@ -146,6 +146,8 @@ class PreNormBlock(nn.Module):
     tuple (branch, residual or None) in place of x gives one: the last addition of a block
     is then made by the next one's norm (sum_of makes it without one)."""
 
+    fused = False
+
     def init_norms(self, cfg, d):
         self.norm1, self.norm2 = norm_of(cfg, d), norm_of(cfg, d)
         self.fused = cfg.get("norm", "layer") == "rms"

@@ -161,6 +161,8 @@ class VisionTransformer(nn.Module):
     num_heads, transformer_units, drop_rate, qkv_bias, K, L, M, num_classes; optional
     norm and linear (RACEBlock)."""
 
+    fused = False  # root-mean-square norms that add the residual
+
     def __init__(self, cfg, attn_type="race", device='cpu'):
         super().__init__()
         if attn_type != "race":

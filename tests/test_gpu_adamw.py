@@ -203,7 +203,8 @@ def test_refusals(dev):
     p = torch.zeros(8, 8, device=dev)
     s = optim.empty_state8(p)
     for a in ([p], [p.t()], [p], [p]), ([p], [p[:4]], [p], [p]), ([p], [p], [p], [p[:, :4]]), ([p, p.to(BF)], [p, p], [p, p], [p, p]), \
-            ([p], [p], [s], [BlockFp8(s.codes, s.scale[:0])]), ([p, p], [p, p], [p, p.clone()], [p, p.clone()]):
+            ([p], [p], [s], [BlockFp8(s.codes, s.scale[:0])]), ([p, p], [p, p], [p, p.clone()], [p, p.clone()]), \
+            ([p], [p.clone()], [p.clone()], [p]):
         with pytest.raises(ValueError):
             optim.adamw_step(*a, step=1, lr=0.1)
     for a in ([p.half()], [p.half()], [p], [p]), ([p], [p], [p.to(BF)], [p]), ([p], [p], [s], [p]), ([p], [p], [p], [s]):
