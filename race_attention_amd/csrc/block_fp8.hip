@@ -689,18 +689,18 @@ __global__ __launch_bounds__(512) void k_block_matmul_few(SkinnyArgs s) {
         }
         return f;
     };
-    constexpr int U = 4;  // blocks of b in flight, and of 16 rows of a
+    // U blocks of b are on their way at once, and of 16 rows of a.  (Whether there is a block is the
+    // wave's own: the branches are uniform.)
+    constexpr int U = 4;
     for (int kb = kb0 + wave; kb < kb1; kb += WAVES * U) {
         i32x8 fb[U];
         uint32_t sb[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int k1 = kb + u * WAVES, kc = k1 < kb1 ? k1 : kb0;
+            const int kc = kb + u * WAVES;
+            if (kc >= kb1) break;
             fb[u] = codes32(brow, (int64_t)kc * BLK + 32 * q);
             sb[u] = sbrow[kc];
-            // behind the wave's last block: zeros times the row's first one, whose NaN are the row's anyway
-            // (no branch below, so that all loads are on their way at once)
-            if (k1 >= kb1) fb[u] = i32x8{0, 0, 0, 0, 0, 0, 0, 0};
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
@@ -710,7 +710,8 @@ __global__ __launch_bounds__(512) void k_block_matmul_few(SkinnyArgs s) {
             uint32_t sa[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int k1 = kb + u * WAVES, kc = k1 < kb1 ? k1 : kb0;
+                const int kc = kb + u * WAVES;
+                if (kc >= kb1) break;
                 const int64_t k = (int64_t)kc * BLK + 32 * q;
                 if constexpr (QUANT) {
                     const TX *row = (const TX *)s.x + mc * s.ldx;
@@ -723,6 +724,7 @@ __global__ __launch_bounds__(512) void k_block_matmul_few(SkinnyArgs s) {
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
+                if (kb + u * WAVES >= kb1) break;
                 if constexpr (QUANT) {
                     float amax = 0.f;
 #pragma unroll
