@@ -45,14 +45,48 @@ template <int L> __device__ __forceinline__ float row_total(float x, float *part
     return x;
 }
 
+// 1 / sqrt(total / D + eps) as a float and what it is short of: the fp32 root, and a step of
+// Newton's in 64 bits.
+__device__ __forceinline__ float row_rstd(float total, double inv_d, float eps, float &low) {
+    const double m = (double)total * inv_d + (double)eps;
+    const float r = 1.f / sqrtf((float)m);
+    const bool number = r > 0.f && r < __builtin_huge_valf();
+    const double d = number ? (double)r * (1.5 - 0.5 * m * (double)r * (double)r) : (double)r;
+    low = number ? (float)(d - (double)(float)d) : 0.f;
+    return (float)d;
+}
+
+// v = v rstd w with one rounding.
+template <int V>
+__device__ __forceinline__ void scale_once(float (&v)[V], float rstd, float low, const float (&w)[V]) {
+    float y[V], sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float p = v[j] * rstd, e = __builtin_fmaf(v[j], low, __builtin_fmaf(v[j], rstd, -p));
+        y[j] = __builtin_fmaf(p, w[j], e * w[j]);
+        sum += y[j];
+    }
+    if (!no_lane(sum != sum)) {  // infinite weights or roots, where e w is no number: the products as they are
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[j] = y[j] == y[j] ? y[j] : v[j] * rstd * w[j];
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = y[j];
+}
+
 // L threads a row, NV vectors of V elements each; NV = 0: any row length, read twice.
 // CODES: y in 8-bit blocks of 128 columns.
+// Where y's roundings show (fp32, and codes, of which those near a tie change), it takes one: three (the
+// root's, shared by the row, and two products') are 5.3e-8 of the norm off, one 3.4e-8, for 3% of the time
+// of 8192 x 4096 (43.3 and 45.4 us).  Rounding to bf16, 1.7e-3, hides them.
+// bf16 with a residual 65536 x 768: 85 us, 4.7 TB/s; to codes 8192 x 4096: 50 us from memory, 4.7 TB/s.
 template <typename TX, typename TR, int V, int NV, int L, bool CODES>
 __global__ __launch_bounds__(NORM_THREADS) void k_rms_norm(NormArgs a) {
     constexpr int RPB = NORM_THREADS / L;
+    constexpr bool ONCE = CODES || std::is_same<TX, float>::value;
     __shared__ float part[4];
     const int t = threadIdx.x % L;
-    const float inv_d = 1.f / (float)a.D;
+    const double inv_d = 1. / (double)a.D;
     const int nv = NV ? NV : (int)((a.D + V * L - 1) / (V * L));
     for (int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / L; row < a.rows; row += (int64_t)gridDim.x * RPB) {
         const TX *x = (const TX *)a.x + row * a.xs;
@@ -82,19 +116,31 @@ __global__ __launch_bounds__(NORM_THREADS) void k_rms_norm(NormArgs a) {
                 for (int j = 0; j < V; ++j) sq += v[0][j] * v[0][j];
             }
         }
-        const float rstd = 1.f / sqrtf(row_total<L>(sq, part) * inv_d + a.eps);
+        const float total = row_total<L>(sq, part);
+        float rstd, low = 0.f;
+        if constexpr (ONCE) rstd = row_rstd(total, inv_d, a.eps, low);
+        else rstd = 1.f / sqrtf(total * (float)inv_d + a.eps);
         if (a.rstd && t == 0) a.rstd[row] = rstd;
         auto store = [&](int i, float(&v)[V]) {
             const int64_t c = ((int64_t)i * L + t) * V;
             if (r) st_row<TR, V>((TR *)a.h + row * a.hs, c, a.D, v);
             float w[V];
             ld_row<float, V>(a.w, c, a.D, w);
+            if constexpr (ONCE) {
+                scale_once<V>(v, rstd, low, w);
+            } else {
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = v[j] * rstd * w[j];
+                for (int j = 0; j < V; ++j) v[j] = v[j] * rstd * w[j];
+            }
             if constexpr (CODES) {
-                float amax = 0.f;
+                float amax = 0.f;  // (NaN are left out by fmaxf)
 #pragma unroll
-                for (int j = 0; j < V; ++j) amax = fmaxf(amax, finite_abs(v[j]));
+                for (int j = 0; j < V; ++j) amax = fmaxf(amax, fabsf(v[j]));
+                if (!no_lane(amax == __builtin_huge_valf())) {
+                    amax = 0.f;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) amax = fmaxf(amax, finite_abs(v[j]));
+                }
                 const int b = scale_byte(lanes<BLK / V>(amax, Max{}));
                 st_codes<V>((uint8_t *)a.y + row * a.ys, c, a.D, v, scale_of(b));
                 if (c % BLK == 0 && c < a.D) a.scale[row * a.ss + c / BLK] = (uint8_t)b;
