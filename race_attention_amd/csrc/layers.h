@@ -54,6 +54,9 @@ template <int V> __device__ __forceinline__ int left_in_row(int64_t c, int64_t n
 template <typename T, int V> __device__ __forceinline__ void ld_raw(const T *row, int64_t c, int64_t n, T (&t)[V]) {
     if (no_lane(c + V > n)) {
         __builtin_memcpy(t, row + c, sizeof t);
+    } else if (no_lane(c < n)) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[j] = (T)0.f;
     } else {
         const int left = left_in_row<V>(c, n);
         const T *p = row + (left ? c : 0);
@@ -75,6 +78,9 @@ template <int V> struct Raw<bf16, V> {
     __device__ __forceinline__ void load(const bf16 *row, int64_t c, int64_t n) {
         if (no_lane(c + V > n)) {
             __builtin_memcpy(w, row + c, sizeof w);
+        } else if (no_lane(c < n)) {
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) w[j] = 0;
         } else {
             const int left = left_in_row<V>(c, n);
             const bf16 *p = row + (left ? c : 0);

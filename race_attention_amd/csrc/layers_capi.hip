@@ -62,8 +62,10 @@ int64_t norm_bwd_grid(int64_t rows, int64_t D) {
     return n < most ? n : most;
 }
 
-// f<V, NV, L>() for a row length: a wave up to 1024 columns, a workgroup up to 16384
-template <typename F> void norm_config(int64_t D, F &&f) {
+// f<V, NV, L>() for a row length: a wave up to 1024 columns, a workgroup up to HELD.  To codes that is 4096:
+// more columns a thread take the registers of the waves that would hide each other's loads (us, 16384 x 5120
+// held and read twice: 188 and 160; 16384 x 8192 239 and 232; 8192 x 16384 509 and 243).
+template <int HELD, typename F> void norm_config(int64_t D, F &&f) {
     const int n = (int)ceil_div(D, 256);
     if (D <= 1024) {
         if (n == 1) f(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 64>{});
@@ -73,9 +75,13 @@ template <typename F> void norm_config(int64_t D, F &&f) {
     } else {
         if (D <= 2048) f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 256>{});
         else if (D <= 4096) f(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, 256>{});
-        else if (D <= 8192) f(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{}, std::integral_constant<int, 256>{});
-        else if (D <= 16384) f(std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{}, std::integral_constant<int, 256>{});
-        else f(std::integral_constant<int, 8>{}, std::integral_constant<int, 0>{}, std::integral_constant<int, 256>{});
+        else {
+            if constexpr (HELD > 4096) {
+                if (D <= 8192) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{}, std::integral_constant<int, 256>{});
+                if (D <= HELD) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{}, std::integral_constant<int, 256>{});
+            }
+            f(std::integral_constant<int, 8>{}, std::integral_constant<int, 0>{}, std::integral_constant<int, 256>{});
+        }
     }
 }
 // f<TX, TR>()
@@ -117,13 +123,12 @@ int norm_forward(const race_norm_desc *d, const void *x, const void *residual, c
     a.eps = d->eps;
     hipStream_t s = (hipStream_t)stream;
     norm_types(d->dtype, residual ? d->r_dtype : d->dtype, [&](auto tx, auto tr) {
-        norm_config(d->D, [&](auto V, auto NV, auto L) {
+        auto launch = [&](auto V, auto NV, auto L, auto to_codes) {
             const unsigned grid = norm_grid(d->rows, NORM_THREADS / L);
-            if (codes)
-                k_rms_norm<decltype(tx), decltype(tr), V, NV, L, true><<<grid, NORM_THREADS, 0, s>>>(a);
-            else
-                k_rms_norm<decltype(tx), decltype(tr), V, NV, L, false><<<grid, NORM_THREADS, 0, s>>>(a);
-        });
+            k_rms_norm<decltype(tx), decltype(tr), V, NV, L, to_codes><<<grid, NORM_THREADS, 0, s>>>(a);
+        };
+        if (codes) norm_config<4096>(d->D, [&](auto V, auto NV, auto L) { launch(V, NV, L, std::true_type{}); });
+        else norm_config<16384>(d->D, [&](auto V, auto NV, auto L) { launch(V, NV, L, std::false_type{}); });
     });
     return launched(what);
 }
@@ -159,14 +164,19 @@ struct MatPlan {
     size_t pack_a, pack_b, parts;  // workspace: repacked operands, parts of a split contraction
 };
 
-// Rows of a up to which k_block_matmul_few multiplies, and up to which it also quantises: every
-// workgroup repeats that, so from 17 rows on a launch of its own is faster (us, 4096 x 4096, 16 rows: 11.5
-// against 14.1; 32: 15.7 and 14.2).  From 33 rows on tiles of 128 are as fast or faster: 64 rows
-// 19 against 17 for 4096 x 4096, 26 against 55 for 8192 x 8192.
+// Rows of a up to which k_block_matmul_few multiplies: beyond them tiles of 128 are as fast or faster (64
+// rows in tiles and as few: 4096 x 4096 19 and 17 us, 8192 x 8192 26 and 55).  And the rows that
+// race_block_linear takes, of 16-bit or 32-bit numbers.
 constexpr int kFewRows = 32, kLinearRows = 16;
 constexpr int kCUs = 256;
 
 bool direct(const race_blocks *b) { return b->ld % 16 == 0 && b->cols % 16 == 0 && (uintptr_t)b->codes % 16 == 0; }
+// Whether the few rows' kernel quantises by itself, or a launch before it does: every workgroup (16 rows
+// of b) repeats the former's work, while the latter costs its launch.  us, the former and the latter, 1 and 16
+// rows, weights from memory, launches of a graph: 768 x 768 3.0 / 4.3, 3.6 / 5.0; 4096 x 4096 7.7 / 8.3,
+// 10.4 / 10.5; 1024 x 8192 9.8 / 9.6, 16.2 / 13.8; 8192 x 4096 14.3 / 12.9, 19.3 / 17.0; 32768 x 1024
+// 19.5 / 17.7, 24.2 / 21.8.
+bool quantise_first(const race_blocks *b) { return b->cols > 4096 || b->rows * b->cols > (1 << 24); }
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 int mat_plan(const race_blocks *a, const race_blocks *b, int out_dtype, MatPlan &p) {
@@ -246,20 +256,43 @@ template <typename TO> void launch_tiles(const MatPlan &p, const MatArgs &m, hip
 template <typename TX, bool QUANT, typename TO>
 void launch_few(const MatPlan &p, const SkinnyArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)p.tn, (unsigned)p.splits);
-    if (QUANT || p.M <= 16) k_block_matmul_few<1, TX, QUANT, TO><<<grid, 512, 0, s>>>(a);
-    else k_block_matmul_few<2, TX, false, TO><<<grid, 512, 0, s>>>(a);
+    if (p.M <= 16) {
+        k_block_matmul_few<1, TX, QUANT, TO><<<grid, 512, 0, s>>>(a);
+    } else if constexpr (!QUANT) {
+        k_block_matmul_few<2, TX, false, TO><<<grid, 512, 0, s>>>(a);
+    }
     if (p.splits > 1) launch_sum<TO>(a.m, p.splits, s);
 }
 
 int check_product(const race_blocks *b, int64_t rows, const float *bias, void *out, int out_dtype, int64_t out_ld,
-                  const MatPlan &p, const void *ws, size_t ws_bytes) {
+                  const MatPlan &p, size_t codes, const void *ws, size_t ws_bytes) {
     int rc;
     if ((rc = check_rows("out", out, esize(out_dtype), rows, b->rows, out_ld, true))) return rc;
     if (bias && (rc = check_ptr("bias", bias, 4))) return rc;
-    const size_t need = p.pack_a + p.pack_b + p.parts;
+    const size_t need = p.pack_a + p.pack_b + p.parts + codes;
     if (need && (!ws || ws_bytes < need)) return fail(RACE_E_WORKSPACE, "workspace %zu bytes < required %zu", ws_bytes, need);
     if (need && (uintptr_t)ws % 16) return fail(RACE_E_INVALID, "workspace is not 16-byte aligned");
     return RACE_OK;
+}
+
+// The codes of a few rows that quantise_first() wants, at ws.
+struct LinearCodes {
+    race_blocks a;
+    size_t bytes;
+};
+LinearCodes linear_codes(int64_t rows, const race_blocks *b, char *ws) {
+    LinearCodes q{};
+    if (!quantise_first(b)) return q;
+    q.a.rows = rows;
+    q.a.cols = b->cols;
+    q.a.ld = round_up(b->cols, 16);
+    q.a.scale_ld = ceil_div(b->cols, BLK);
+    q.a.block_rows = 1;
+    const size_t codes = align256((size_t)(rows * q.a.ld));
+    q.a.codes = ws;
+    q.a.scale = ws ? ws + codes : nullptr;
+    q.bytes = codes + align256((size_t)(rows * q.a.scale_ld));
+    return q;
 }
 
 MatArgs mat_args(const MatPlan &p, const race_blocks *a, const race_blocks *b, const float *bias, void *out,
@@ -358,7 +391,7 @@ int race_rms_norm_bwd(const race_norm_desc *d, const void *x, const void *residu
     a.drs = d->dr_stride;
     hipStream_t s = (hipStream_t)stream;
     norm_types(d->dtype, d->r_dtype, [&](auto tx, auto tr) {
-        norm_config(d->D, [&](auto V, auto NV, auto L) {
+        norm_config<16384>(d->D, [&](auto V, auto NV, auto L) {
             k_rms_norm_bwd<decltype(tx), decltype(tr), V, NV, L><<<(unsigned)grid, NORM_THREADS, 0, s>>>(a);
         });
     });
@@ -451,7 +484,7 @@ int race_block_matmul(const race_blocks *a, const race_blocks *b, const float *b
                       int64_t out_ld, void *ws, size_t ws_bytes, void *stream) {
     MatPlan p;
     int rc;
-    if ((rc = mat_plan(a, b, out_dtype, p)) || (rc = check_product(b, a->rows, bias, out, out_dtype, out_ld, p, ws, ws_bytes)))
+    if ((rc = mat_plan(a, b, out_dtype, p)) || (rc = check_product(b, a->rows, bias, out, out_dtype, out_ld, p, 0, ws, ws_bytes)))
         return rc;
     SkinnyArgs sk{};
     MatArgs &m = sk.m;
@@ -497,9 +530,12 @@ size_t race_block_linear_workspace_bytes(int64_t rows, const race_blocks *b, int
         fail(RACE_E_INVALID, "1 to %d rows (got %lld) and a matrix b", kLinearRows, (ll)rows);
         return 0;
     }
+    MatPlan p;
     race_blocks a = *b;
     a.rows = rows;
-    return race_block_matmul_workspace_bytes(&a, b, out_dtype);
+    if (mat_plan(&a, b, out_dtype, p)) return 0;
+    ok();
+    return p.parts + linear_codes(rows, b, nullptr).bytes;
 }
 
 int race_block_linear(const void *x, int32_t dtype, int64_t rows, int64_t x_ld, const race_blocks *b, const float *bias,
@@ -513,19 +549,23 @@ int race_block_linear(const void *x, int32_t dtype, int64_t rows, int64_t x_ld, 
     race_blocks a = *b;  // sizes alone: x takes its codes' place
     a.rows = rows;
     MatPlan p;
-    if ((rc = mat_plan(&a, b, out_dtype, p)) || (rc = check_product(b, rows, bias, out, out_dtype, out_ld, p, ws, ws_bytes))) return rc;
+    if ((rc = mat_plan(&a, b, out_dtype, p)) ||
+        (rc = check_product(b, rows, bias, out, out_dtype, out_ld, p, linear_codes(rows, b, nullptr).bytes, ws, ws_bytes)))
+        return rc;
+    const LinearCodes q = linear_codes(rows, b, (char *)ws + p.parts);
+    if (q.bytes) {
+        if ((rc = race_quantize(x, dtype, rows, b->cols, x_ld, &q.a, nullptr, nullptr, nullptr, 0, stream))) return rc;
+        a = q.a;
+    }
     SkinnyArgs sk{};
     sk.m = mat_args(p, &a, b, bias, out, out_ld, ws);
     sk.x = x;
     sk.ldx = x_ld;
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == RACE_DTYPE_BF16) {
-        if (out_dtype == RACE_DTYPE_BF16) launch_few<bf16, true, bf16>(p, sk, s);
-        else launch_few<bf16, true, float>(p, sk, s);
-    } else {
-        if (out_dtype == RACE_DTYPE_BF16) launch_few<float, true, bf16>(p, sk, s);
-        else launch_few<float, true, float>(p, sk, s);
-    }
+    const bool f32 = out_dtype == RACE_DTYPE_F32;
+    if (q.bytes) f32 ? launch_few<bf16, false, float>(p, sk, s) : launch_few<bf16, false, bf16>(p, sk, s);
+    else if (dtype == RACE_DTYPE_BF16) f32 ? launch_few<bf16, true, float>(p, sk, s) : launch_few<bf16, true, bf16>(p, sk, s);
+    else f32 ? launch_few<float, true, float>(p, sk, s) : launch_few<float, true, bf16>(p, sk, s);
     return launched("race_block_linear");
 }
 

@@ -12,7 +12,7 @@
 // Bound by memory: every array is read or written once.  A row is held in registers by
 // one wave (up to 1024 columns, four rows a workgroup, so that no barrier is needed and
 // a decode batch of a few rows still starts as many workgroups) or by a workgroup of
-// 256 threads (up to 16384 columns); longer rows are read twice.  Vectors start at
+// 256 threads (up to 16384 columns, 4096 to codes); longer rows are read twice.  Vectors start at
 // any address (an odd row length shifts every row).
 #include "layers.h"
 
@@ -123,6 +123,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_rms_norm(NormArgs a) {
         if (a.rstd && t == 0) a.rstd[row] = rstd;
         auto store = [&](int i, float(&v)[V]) {
             const int64_t c = ((int64_t)i * L + t) * V;
+            if (no_lane(c < a.D)) return;
             if (r) st_row<TR, V>((TR *)a.h + row * a.hs, c, a.D, v);
             float w[V];
             ld_row<float, V>(a.w, c, a.D, w);

@@ -211,6 +211,24 @@ def test_linear_layer_and_its_gradients(dev, xdt, wdt, bias, shape, N):
         assert torch.equal(got, (dx, dw, *db)[i])
 
 
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("R,N,K", [(1, 768, 768), (16, 96, 1000), (1, 16, 4096), (1, 16, 4097), (5, 300, 5000),
+                                   (16, 4096, 4096), (16, 4112, 4096), (3, 33000, 520), (17, 100, 4100)])
+def test_rows_quantised_inside_or_before_the_product(dev, dt, R, N, K):
+    """A serving call's rows have the quantiser's codes, wherever they are formed: the product of its codes, bit for
+    bit; the last row of a larger batch of the same kernel too, and rows with a pitch."""
+    g = torch.Generator().manual_seed(N + K)
+    x = (torch.randn(R, K, generator=g) * torch.exp2(torch.randint(-9, 9, (R, K), generator=g).float())).to(dt).to(dev)
+    w = fp8.quantize(torch.randn(N, K, generator=g).to(dev), 128)
+    bias = torch.randn(N, generator=g).to(dev)
+    with torch.no_grad():
+        y = fp8.linear(x, w, bias)
+        assert torch.equal(y, fp8.matmul(fp8.quantize(x), w, bias=bias, out_dtype=dt))
+        wide = torch.full((R, K + 24), float("nan"), dtype=dt, device=dev)
+        wide[:, :K] = x
+        assert torch.equal(fp8.linear(wide[:, :K], w, bias), y)
+
+
 def test_linear_gradient_follows_differences(dev):
     """The 8-bit gradients are those of the layer up to the rounding of their operands to e4m3: a product
     of two operands that are each at most 2^-4 off per value is 2^-3 (1 + 2^-5) of the sum of magnitudes off."""

@@ -130,7 +130,7 @@ def test_gradient_against_differences(dev):
 
 @pytest.mark.parametrize("dt,rdt", [(BF, None), (BF, BF), (BF, F32), (F32, F32)])
 @pytest.mark.parametrize("rows,D", [(1, 1), (3, 64), (5, 100), (9, 128), (4, 768), (3, 1001), (2, 1300), (3, 4096),
-                                    (2, 8200), (1, 20000), (300, 384)])
+                                    (2, 8200), (1, 20000), (300, 384), (5, 4097), (2, 7000)])
 def test_output_in_8_bits(dev, dt, rdt, rows, D):
     x, r, w, _, _ = make(rows, D, dt, rdt, seed=D)
     y = norm.rms_norm_fp8(x.to(dev), w.to(dev), residual=None if r is None else r.to(dev), eps=EPS)
@@ -182,6 +182,36 @@ def test_strides(dev):
     dx, = torch.autograd.grad(y.sum(), x)  # an expanded gradient: stride 0
     check_backward(x.detach().cpu(), None, w.cpu(), torch.ones(x.shape, dtype=BF), None, dx, None,
                    torch.autograd.grad(norm.rms_norm(x, w.requires_grad_(True)).sum(), w)[0])
+
+
+@pytest.mark.parametrize("D", [64, 768, 1300, 6000])
+@pytest.mark.parametrize("eight", [False, True])
+def test_infinite_weights_and_roots(dev, D, eight):
+    """An infinite weight, and a row whose squares are under the smallest number (eps 0): the products' infinities,
+    NaN where they are 0 times infinity, and the columns and rows beside them as they were."""
+    g = torch.Generator().manual_seed(D)
+    x, w = torch.randn(4, D, generator=g), torch.ones(D)
+    x[1] *= 1e-30
+    x[2, 5] = 0
+    w[5] = float("inf")
+    w[9] = -float("inf")
+
+    def norm_of(x, w):
+        if not eight:
+            return norm.rms_norm(x.to(dev), w.to(dev), eps=0.0).cpu()
+        q = norm.rms_norm_fp8(x.to(dev), w.to(dev), eps=0.0)
+        return q.dequantize().float().cpu()
+
+    y, rest = norm_of(x, w), norm_of(x[[0, 2, 3]], torch.ones(D))
+    keep = [c for c in range(D) if c not in (5, 9)]
+    if eight:  # infinities have no code, and the largest finite value decides the scale
+        assert torch.isnan(y[1]).all() and torch.isnan(y[:, [5, 9]]).all()
+        assert torch.isfinite(y[[0, 2, 3]][:, keep]).all()
+    else:
+        assert torch.equal(y[1, keep], torch.copysign(torch.full((D - 2,), float("inf")), x[1, keep]))
+        assert torch.isnan(y[2, 5]) and y[0, 5] == torch.sign(x[0, 5]) * float("inf")
+        assert y[3, 9] == -torch.sign(x[3, 9]) * float("inf")
+        assert torch.equal(y[[0, 2, 3]][:, keep], rest[:, keep])
 
 
 def test_empty(dev):

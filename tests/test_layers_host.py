@@ -103,6 +103,11 @@ def test_product_refusals():
                                  None) == -2
     assert lib.race_block_linear(P, 3, 1, 512, r(_blocks()), None, P, 1, 256, P, 1 << 30, None) == -1
     assert lib.race_block_linear_workspace_bytes(0, r(_blocks()), 1) == 0
+    wide = _blocks(256, 8192)  # rows of x are quantised into the workspace first
+    need = lib.race_block_linear_workspace_bytes(16, r(wide), 1)
+    assert need >= 16 * (8192 + 64)
+    assert lib.race_block_linear(P, 1, 16, 8192, r(wide), None, P, 1, 256, None, 0, None) == -3
+    assert lib.race_block_linear(P, 1, 16, 8192, r(wide), None, P, 1, 256, P, need - 1, None) == -3
     long = _blocks(300, 1 << 23)
     assert lib.race_block_matmul(r(long), r(long), None, P, 1, 300, P, 1 << 40, None) == -2 and "2^22" in _lib.last_error()
 
