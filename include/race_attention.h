@@ -315,8 +315,9 @@ size_t race_block_matmul_workspace_bytes(const race_blocks *a, const race_blocks
 int race_block_matmul(const race_blocks *a, const race_blocks *b, const float *bias, void *out,
                       int32_t out_dtype, int64_t out_ld, void *ws, size_t ws_bytes, void *stream);
 
-/* The same for 1 to race_block_linear_rows() rows of x in bf16 or fp32, quantised on the way as
- * race_quantize with block_rows = 1 does: a linear layer's single tokens in one launch. */
+/* The same for 1 to race_block_linear_rows() rows of x in bf16 or fp32, quantised as race_quantize
+ * with block_rows = 1 does: a linear layer's single tokens.  Small b: in one launch; others: in the
+ * workspace first. */
 int64_t race_block_linear_rows(void);
 size_t race_block_linear_workspace_bytes(int64_t rows, const race_blocks *b, int32_t out_dtype);
 int race_block_linear(const void *x, int32_t dtype, int64_t rows, int64_t x_ld, const race_blocks *b,

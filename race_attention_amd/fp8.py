@@ -11,7 +11,8 @@ about 2e-5 of the sum's norm off.
 is differentiable: the forward quantises x (a scale for 128 columns of a row) and the weight (for
 128 x 128), the backward dy likewise, and dx = dy W and dW = dy^T x are 8-bit products
 too, of operands quantised along the contraction.  With a BlockFp8 as the weight it serves:
-up to 16 rows of x, such as single tokens, are one launch.  ``Linear`` is the module,
+up to 16 rows of x, such as single tokens, are quantised inside the product where the weight
+is small enough that this pays.  ``Linear`` is the module,
 ``Linear.freeze()`` turns its weight into a BlockFp8 once.
 """
 from __future__ import annotations
