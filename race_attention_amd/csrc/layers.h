@@ -37,6 +37,16 @@ template <typename T, int V> __device__ __forceinline__ void st_vec(T *p, const 
     for (int j = 0; j < V; ++j) t[j] = (T)r[j];
     __builtin_memcpy(p, t, sizeof t);
 }
+// The bytes of t, 8 or 16, to any address, as data that this launch does not touch again.  The caches then give up
+// lines that are read again less often (us: product 50240 x 1536, K = 384, 82 and 69; norm forward and
+// backward of 65536 x 768 191 and 173).  Lanes must fill lines together: 32 bytes a lane, in two stores, are
+// slower so (fp32 8192 x 16384: 407 and 508), and stay as they were.
+template <typename A> __device__ __forceinline__ void st_stream(void *p, const A &t) {
+    typedef int words __attribute__((ext_vector_type(sizeof(A) / 4), aligned(1)));
+    words w;
+    __builtin_memcpy(&w, &t, sizeof w);
+    __builtin_nontemporal_store(w, (words *)p);
+}
 // whether a condition holds in none of the wave's active lanes: a branch on it is the wave's, so its
 // other side costs nothing
 __device__ __forceinline__ bool no_lane(bool x) { return __builtin_amdgcn_ballot_w64(x) == 0; }
@@ -104,7 +114,11 @@ template <typename T, int V> __device__ __forceinline__ void ld_row(const T *row
 }
 template <typename T, int V> __device__ __forceinline__ void st_row(T *row, int64_t c, int64_t n, const float (&r)[V]) {
     if (c + V <= n) {
-        st_vec<T, V>(row + c, r);
+        T t[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[j] = (T)r[j];
+        if constexpr (sizeof t <= 16) st_stream(row + c, t);
+        else __builtin_memcpy(row + c, t, sizeof t);
     } else {
 #pragma unroll
         for (int j = 0; j < V; ++j)
