@@ -126,8 +126,9 @@ template <typename T> __global__ __launch_bounds__(256) void k_quantize_rows(Qua
 // then over the 16 threads above each other through LDS.  Transposed codes leave through
 // LDS in rows of 128 bytes: word w (4 rows) of a column stands at w ^ swizzle(column), so
 // that neither the 16 columns 8 apart of a write nor a read's pieces of 8 columns meet in a bank.
-// Bound by memory: bf16 50240 x 1536 both ways and its sums, from memory, 69 us (4.5 TB/s); a call for each
-// of the three would read x three times.  fp32 1536 x 384 as 128 x 128 blocks both ways: 6.8 us, 36
+// Bound by memory: bf16 50240 x 1536 both ways and its sums, from memory, 65 us (4.8 TB/s); a call for each
+// of the three would read x three times.  (Codes past the caches: 300 us for a layer's forward and backward that
+// takes 290, whose products read them next.)  fp32 1536 x 384 as 128 x 128 blocks both ways: 6.8 us, 36
 // workgroups' latency.
 template <typename T, bool BLOCK>
 __global__ __launch_bounds__(256) void k_quantize_tile(QuantArgs a) {
@@ -398,9 +399,9 @@ __device__ __forceinline__ void tile_of(int id, int tm, int tn, int &im, int &in
 // loads and reads are issued between matrix instructions, which hide them.  Scales are fetched 16
 // steps at a time (a row's 16 bytes; every fetch costs a line of the L1) and read from LDS step by step.
 // The outputs leave through LDS in whole rows.
-// Bound by the matrix cores where the contraction is long: 8192^3 386-420 us, 2.6-2.85 PFLOP/s (0.88-0.97 of
+// Bound by the matrix cores where the contraction is long: 8192^3 400-417 us, 2.6-2.75 PFLOP/s (0.89-0.93 of
 // the library's 8-bit product with one scale a tensor); 4096^3 57 us, 2.4.  Short contractions are bound by the
-// tile's beginning and end: 50240 x 1536, K = 384, 64 us, 0.9.  fp32 outputs 4096^3 118 us, 1.17 (the
+// tile's beginning and end: 50240 x 1536, K = 384, 72 us, 0.82, of which the outputs' bytes are 30.  fp32 outputs 4096^3 118 us, 1.17 (the
 // library's bf16 product 1.34-1.46).
 template <int BM, int BN, int WM, int WN, typename TO>
 __global__ __launch_bounds__(64 * WM * WN, 1) void k_block_matmul(MatArgs a) {

@@ -207,12 +207,13 @@ int mat_plan(const race_blocks *a, const race_blocks *b, int out_dtype, MatPlan 
             return fail(RACE_E_UNSUPPORTED, "row pitch of 2^22 bytes or more (a %lld, b %lld)", (ll)lda, (ll)ldb);
         // Tiles of 256 x 256 (one workgroup a CU) feed the matrix cores better, 1.6 us a step
         // against 2 x 1.0 us of the four times smaller work of 128 x 128 (two a CU); but no other workgroup
-        // works while one begins and ends, 12 us against 4.  128 x 128 may also split the contraction;
+        // works while one begins and ends, 10 us against 4.  128 x 128 may also split the contraction;
         // its parts are written and read once (4 TB/s) and take a launch.  The least estimate is taken.
-        // us, 256 and 128: 8192^3 402 and 493; 4096^3 59 and 65; 50240 x 1536, K = 384, 82 and 64;
-        // 8192 x 2304, K = 768, 40 and 28.  (fp32 outputs: the bf16 operands take 128 x 128's registers.)
+        // us, 256 and 128: 8192^3 398 and 495; 4096^3 57 and 66; 4096 x 4096, K = 1024, 23.4 and 25.8; 50240 x 1536,
+        // K = 384, 75 and 72; 50240 x 384, K = 1536, 53 and 45; 8192 x 2304, K = 768, 35 and 28; 2048 x 2048, K =
+        // 8192, split, 79 and 46.  (fp32 outputs: the bf16 operands take 128 x 128's registers.)
         const int64_t big = ceil_div(p.M, 256) * ceil_div(p.N, 256), small = ceil_div(p.M, 128) * ceil_div(p.N, 128);
-        double best = out_dtype == RACE_DTYPE_F32 ? 1e30 : (double)ceil_div(big, kCUs) * (1.6 * p.ksteps + 12);
+        double best = out_dtype == RACE_DTYPE_F32 ? 1e30 : (double)ceil_div(big, kCUs) * (1.6 * p.ksteps + 10);
         p.bm = 256;
         for (int s = 1; s == 1 || (s <= 64 && 2 * s <= p.ksteps && (s - 1) * small < 2 * kCUs); ++s) {
             const int64_t wgs = small * s;

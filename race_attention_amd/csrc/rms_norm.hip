@@ -79,7 +79,7 @@ __device__ __forceinline__ void scale_once(float (&v)[V], float rstd, float low,
 // Where y's roundings show (fp32, and codes, of which those near a tie change), it takes one: three (the
 // root's, shared by the row, and two products') are 5.3e-8 of the norm off, one 3.4e-8, for 3% of the time
 // of 8192 x 4096 (43.3 and 45.4 us).  Rounding to bf16, 1.7e-3, hides them.
-// bf16 with a residual 65536 x 768: 85 us, 4.7 TB/s; to codes 8192 x 4096: 50 us from memory, 4.7 TB/s.
+// bf16 with a residual 65536 x 768: 83 us, 4.9 TB/s; to codes 8192 x 4096: 47 us, 5.0 TB/s (a large copy: 5.1).
 template <typename TX, typename TR, int V, int NV, int L, bool CODES>
 __global__ __launch_bounds__(NORM_THREADS) void k_rms_norm(NormArgs a) {
     constexpr int RPB = NORM_THREADS / L;
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(NORM_THREADS) void k_rms_norm(NormArgs a) {
 // A row is a chain of loads, a sum over its lanes and stores; AHEAD (rows of few registers): the next
 // row's loads are on their way meanwhile, and w stays in registers (8192 x 4096 bf16 with a residual:
 // 85 us without, 67 with).  bf16 waits in pairs: as single values it took a register each, and 65536 x
-// 768 with a residual 163 us; it takes 100, 5.0 TB/s.
+// 768 with a residual 163 us; it takes 88 (dx past the caches; 105 through them).
 template <typename TX, typename TR, int V, int NV, int L>
 __global__ __launch_bounds__(NORM_THREADS) void k_rms_norm_bwd(NormArgs a) {
     constexpr int RPB = NORM_THREADS / L, N = NV ? NV : 1;
