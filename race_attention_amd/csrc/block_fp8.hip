@@ -399,7 +399,7 @@ __device__ __forceinline__ void tile_of(int id, int tm, int tn, int &im, int &in
 // loads and reads are issued between matrix instructions, which hide them.  Scales are fetched 16
 // steps at a time (a row's 16 bytes; every fetch costs a line of the L1) and read from LDS step by step.
 // The outputs leave through LDS in whole rows.
-// Bound by the matrix cores where the contraction is long: 8192^3 400-417 us, 2.6-2.75 PFLOP/s (0.89-0.93 of
+// Bound by the matrix cores where the contraction is long: 8192^3 400-428 us, 2.6-2.75 PFLOP/s (0.87-0.93 of
 // the library's 8-bit product with one scale a tensor); 4096^3 57 us, 2.4.  Short contractions are bound by the
 // tile's beginning and end: 50240 x 1536, K = 384, 72 us, 0.82, of which the outputs' bytes are 30.  fp32 outputs 4096^3 118 us, 1.17 (the
 // library's bf16 product 1.34-1.46).
